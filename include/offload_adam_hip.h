@@ -361,6 +361,48 @@ int oa_adam_requant_nvfp4(const void* grad, void* exp_avg, void* exp_avg_sq,
                           void* workspace, void* stream);
 
 /* ------------------------------------------------------------------------
+ * E. Loss of a linear head.  No counterpart in the reference, whose example
+ * computes logits and calls cross_entropy on them (examples/e2e_train/train.py).
+ *
+ *   z = x w^T (never stored),  loss_t = log sum_v exp z[t,v] - z[t,target_t]
+ *
+ *   x        [tokens][hidden] bf16 or f16, rows ldx elements apart
+ *   w        [vocab][hidden] of the same type, rows ldw elements apart
+ *            (hidden, ldx, ldw multiples of 8, both 16-byte aligned, else OA_EALIGN)
+ *   target   int64[tokens]; ignore_index: the token takes no part (loss and
+ *            gradients 0, whatever its row of x holds); any other value outside
+ *            [0, vocab) makes the token's loss and its gradients NaN
+ *   loss     f32: one element (mean over the tokens that take part, NaN if there
+ *            are none; or sum), or [tokens] (none)
+ *   lse      f32[tokens], count f32[1]: for the backward pass
+ *   workspace  oa_linear_ce_workspace_bytes() bytes, 256-byte aligned, used until
+ *            the enqueued work has run
+ * Sizes: hidden strides up to 2^20 elements, 2^22 tokens, 2^24 rows of w.
+ * ---------------------------------------------------------------------- */
+#define OA_LOSS_NONE 0
+#define OA_LOSS_MEAN 1
+#define OA_LOSS_SUM  2
+
+/* backward = 0: of the forward pass (want_* unused); else of the backward pass that
+ * computes dx and / or dw.  0 for sizes out of range. */
+size_t oa_linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab,
+                                    int backward, int want_dx, int want_dw);
+
+int oa_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                         const int64_t* target, int64_t tokens, int64_t hidden,
+                         int64_t vocab, int64_t ignore_index, int reduction, float* loss,
+                         float* lse, float* count, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* dx [tokens][hidden] and dw [vocab][hidden], contiguous, in the type of x and w;
+ * either may be NULL.  grad: f32, of loss's shape.  tokens > 0. */
+int oa_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                          const int64_t* target, int64_t tokens, int64_t hidden,
+                          int64_t vocab, int64_t ignore_index, int reduction,
+                          const float* lse, const float* count, const float* grad, void* dx,
+                          void* dw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * D. Pinned host memory and host<->device streaming.
  * ---------------------------------------------------------------------- */
 

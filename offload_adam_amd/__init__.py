@@ -3,7 +3,8 @@ with every kernel hand-written in HIP for AMD Instinct MI355X (gfx950).
 
 Public surface mirrors the reference package ``offload_adam``: ``Adam`` and
 ``OffloadAdam`` (plus ``offload_adam_amd.kernels`` and
-``offload_adam_amd.qweight``).
+``offload_adam_amd.qweight``); ``linear_cross_entropy`` is the loss of a model's
+output layer without its logits.
 """
 
 from . import _runtime_env
@@ -14,6 +15,7 @@ from . import _runtime_env
 _runtime_env.prepare()
 
 from .adam import Adam  # noqa: E402
+from .loss import linear_cross_entropy  # noqa: E402
 from .offload_adam import OffloadAdam  # noqa: E402
 
 __version__ = "0.1.0"
@@ -30,4 +32,4 @@ class DistributedOffloadAdam(OffloadAdam):
         )
 
 
-__all__ = ["Adam", "OffloadAdam", "DistributedOffloadAdam"]
+__all__ = ["Adam", "OffloadAdam", "DistributedOffloadAdam", "linear_cross_entropy"]

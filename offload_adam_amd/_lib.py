@@ -123,6 +123,21 @@ SIGNATURES = {
         [c_void_p] * 4 + [c_int64] + _ADAM_TAIL
         + [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    # tokens, hidden, vocab, backward, want_dx, want_dw
+    "oa_linear_ce_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 3),
+    # x, ldx, w, ldw, dtype, target, tokens, hidden, vocab, ignore_index, reduction,
+    # loss, lse, count, workspace, workspace_bytes, stream
+    "oa_linear_ce_forward": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p] + [c_int64] * 4
+        + [c_int] + [c_void_p] * 4 + [c_size_t, c_void_p],
+    ),
+    # as above up to reduction; lse, count, grad, dx, dw, workspace, workspace_bytes, stream
+    "oa_linear_ce_backward": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p] + [c_int64] * 4
+        + [c_int] + [c_void_p] * 6 + [c_size_t, c_void_p],
+    ),
     "oa_pinned_alloc": (
         c_int,
         [c_size_t, c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int)],
@@ -151,6 +166,7 @@ OA_EOS = -5
 OA_EUNAVAILABLE = -6
 OA_COPY_H2D, OA_COPY_D2H, OA_COPY_D2D = 0, 1, 2
 OA_F32, OA_BF16, OA_F16 = 0, 1, 2
+OA_LOSS_NONE, OA_LOSS_MEAN, OA_LOSS_SUM = 0, 1, 2
 
 
 def dtype_code(dtype):

@@ -1,0 +1,151 @@
+"""Cross entropy of a linear output layer, without its logits.
+
+The logits of a language model are the largest tensor of its training step: 4096
+tokens of the 8B model are 1 GB in bf16, 2.1 GB in the fp32 that the loss needs, and
+as much again for their gradient.  ``linear_cross_entropy`` takes the hidden states
+and the output layer's weight instead; HIP kernels fold each tile of logits into a
+running maximum and sum while it is in registers and compute it again for the
+gradients.  The reference has no counterpart: its example's model returns logits
+(examples/e2e_train/train.py).
+"""
+
+from ctypes import c_int, c_int64, c_size_t
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .qweight import base as _qbase
+
+_REDUCTIONS = {"none": _lib.OA_LOSS_NONE, "mean": _lib.OA_LOSS_MEAN, "sum": _lib.OA_LOSS_SUM}
+
+
+def _rows(t, name):
+    """2-D operand of the kernels: unit column stride, columns and row stride multiples
+    of 8 elements, 16-byte aligned.  Anything else is copied, zero-padded."""
+    rows, cols = t.shape
+    stride = t.stride(0) if rows > 1 else -(-cols // 8) * 8
+    if (cols % 8 == 0 and (cols == 1 or t.stride(1) == 1) and stride >= cols and stride % 8 == 0
+            and stride <= 1 << 20 and t.data_ptr() % 16 == 0):
+        return t, cols, stride
+    padded = -(-cols // 8) * 8
+    out = torch.zeros((rows, padded), dtype=t.dtype, device=t.device)
+    out[:, :cols].copy_(t)
+    return out, padded, padded
+
+
+def _plain(weight, dtype):
+    if isinstance(weight, _qbase.QWeightBase):
+        return _qbase._dequantized(weight, dtype)
+    return weight
+
+
+def _head_args(x, w, target, ignore_index, reduction):
+    x, hidden, ldx = _rows(x, "x")
+    w, _, ldw = _rows(w, "weight")
+    args = [_lib.ptr(x), c_int64(ldx), _lib.ptr(w), c_int64(ldw),
+            c_int(_lib.dtype_code(x.dtype)), _lib.ptr(target), c_int64(x.shape[0]),
+            c_int64(hidden), c_int64(w.shape[0]), c_int64(ignore_index),
+            c_int(_REDUCTIONS[reduction])]
+    return args, hidden, (x, w)
+
+
+def _workspace(device, tokens, hidden, vocab, backward, dx, dw):
+    nbytes = _lib.load().oa_linear_ce_workspace_bytes(
+        c_int64(tokens), c_int64(hidden), c_int64(vocab), c_int(backward), c_int(dx), c_int(dw))
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index, reduction):
+        dev, tokens = x.device, x.shape[0]
+        lib = _lib.load()
+        with _lib.device_guard(dev):
+            w = _plain(weight, x.dtype)
+            args, hidden, keep = _head_args(x, w, target, ignore_index, reduction)
+            loss = torch.empty((tokens,) if reduction == "none" else (), dtype=torch.float32,
+                               device=dev)
+            lse = torch.empty(max(tokens, 1), dtype=torch.float32, device=dev)
+            count = torch.empty(1, dtype=torch.float32, device=dev)
+            if loss.numel():
+                ws = _workspace(dev, tokens, hidden, w.shape[0], 0, 0, 0)
+                code = lib.oa_linear_ce_forward(
+                    *args, _lib.ptr(loss), _lib.ptr(lse), _lib.ptr(count), _lib.ptr(ws),
+                    c_size_t(ws.numel()), _lib.current_stream_ptr())
+                _lib.check(code, "oa_linear_ce_forward")
+        ctx.save_for_backward(x, weight, target, lse, count)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, target, lse, count = ctx.saved_tensors
+        want_dx, want_dw = ctx.needs_input_grad[:2]
+        tokens, dev = x.shape[0], x.device
+        if tokens == 0:
+            return (torch.zeros_like(x) if want_dx else None,
+                    torch.zeros(weight.shape, dtype=x.dtype, device=dev) if want_dw else None,
+                    None, None, None)
+        lib = _lib.load()
+        with _lib.device_guard(dev):
+            w = _plain(weight, x.dtype)
+            args, hidden, keep = _head_args(x, w, target, ctx.ignore_index, ctx.reduction)
+            vocab = w.shape[0]
+            grad = grad.contiguous()
+            dx = torch.empty((tokens, hidden), dtype=x.dtype, device=dev) if want_dx else None
+            dw = torch.empty((vocab, hidden), dtype=x.dtype, device=dev) if want_dw else None
+            ws = _workspace(dev, tokens, hidden, vocab, 1, int(want_dx), int(want_dw))
+            code = lib.oa_linear_ce_backward(
+                *args, _lib.ptr(lse), _lib.ptr(count), _lib.ptr(grad), _lib.ptr(dx),
+                _lib.ptr(dw), _lib.ptr(ws), c_size_t(ws.numel()), _lib.current_stream_ptr())
+            _lib.check(code, "oa_linear_ce_backward")
+            if hidden != x.shape[1]:  # operands were padded
+                dx = dx[:, :x.shape[1]].contiguous() if want_dx else None
+                dw = dw[:, :x.shape[1]].contiguous() if want_dw else None
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean"):
+    """``F.cross_entropy(F.linear(x, weight).float(), target)`` without the logits.
+
+    ``x``: hidden states (..., hidden), bf16 or fp16, on the GPU; ``weight``: the output
+    layer's (vocab, hidden) in the same dtype, or a quantised weight of this package
+    (decoded for the call); ``target``: int64 of ``x``'s leading shape.  Tokens whose
+    target is ``ignore_index`` take no part: their losses and gradients are 0, whatever
+    their rows of ``x`` hold.  Any other target outside [0, vocab) gives NaN.
+
+    ``reduction``: ``"mean"`` over the tokens that take part (NaN if there are none),
+    ``"sum"``, or ``"none"`` (losses of ``target``'s shape).  The loss is fp32;
+    logits, exponentials and sums are fp32 throughout, and only the logits' gradient is
+    rounded to 16 bits, once, between the two products that use it.  Gradients flow to
+    ``x`` and ``weight``; second derivatives are not available.  Results do not depend
+    on anything but the arguments: no atomics, one order of summation.
+
+    Works on ``x``'s device and the current stream, synchronises nothing, and may be
+    captured into a graph (with the backward pass inside the same capture).
+    """
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
+        raise TypeError("x and weight must be tensors")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if weight.dtype != x.dtype:
+        raise TypeError(f"weight must have x's dtype {x.dtype}, got {weight.dtype}")
+    if not isinstance(target, torch.Tensor) or target.dtype != torch.int64:
+        raise TypeError("target must be an int64 tensor")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target has shape {tuple(target.shape)}, expected {tuple(x.shape[:-1])}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError("weight must not be empty")
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor (no CPU path exists)")
+    if weight.device != x.device or target.device != x.device:
+        raise ValueError("x, weight and target must be on the same GPU")
+    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight,
+                                     target.reshape(-1).contiguous(), int(ignore_index), reduction)
+    return loss.reshape(target.shape) if reduction == "none" else loss
