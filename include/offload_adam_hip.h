@@ -403,6 +403,47 @@ int oa_linear_ce_backward(const void* x, int64_t ldx, const void* w, int64_t ldw
                           void* dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * F. 8-bit floating-point weights with block scales, and the linear layer on them.
+ * No counterpart in the reference, whose formats are weight-only.
+ *
+ *   q        e4m3[out_features][in_features], in_features a multiple of 16,
+ *            16-byte aligned
+ *   scales   e8m0[ceil(out_features / 128)][ceil(in_features / 128)]: the smallest
+ *            power of two (2^-126 at least) that brings the largest finite magnitude
+ *            of its 128 x 128 block to 448 or less, 1 for a block of zeros;
+ *            code = e4m3(element / scale), to nearest even, NaN if not finite
+ * ---------------------------------------------------------------------- */
+
+int oa_quant_fp8(const void* src, int src_dtype, int64_t src_row_stride, int64_t rows,
+                 int64_t cols, void* q, void* scales, void* stream);
+
+/* out = code * scale, rounded to out_dtype (exact but for fp16's range). */
+int oa_dequant_fp8(const void* q, const void* scales, int64_t rows, int64_t cols, void* out,
+                   int out_dtype, int64_t out_row_stride, void* stream);
+
+/* 0 for sizes that are not positive.  backward = 0: want_* unused. */
+size_t oa_fp8_linear_workspace_bytes(int64_t tokens, int64_t in_features,
+                                     int64_t out_features, int backward, int want_dx,
+                                     int want_dw, int want_db);
+
+/* y = xq w^T + bias: x [tokens][in_features] (f32, bf16 or f16 by `dtype`, rows ldx
+ * elements apart) is encoded as w is, in blocks of 1 x 128 along its rows; fp32 sums,
+ * one rounding of the sum with the bias to `dtype`.  y contiguous; bias in `dtype`,
+ * NULL for none.  The workspace is 256-byte aligned.  Up to 2^22 tokens and features. */
+int oa_fp8_linear_forward(const void* x, int64_t ldx, int dtype, int64_t tokens,
+                          const void* q, const void* scales, const void* bias,
+                          int64_t out_features, int64_t in_features, void* y,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* dx = gq w (the gradient encoded in blocks of 1 x 128 along its rows), dw = gt^T xt
+ * (gradient and x encoded in blocks of 128 tokens of a column), db = the columns' sums
+ * of the gradient itself.  Contiguous, in `dtype`; any may be NULL. */
+int oa_fp8_linear_backward(const void* grad, int64_t ldg, const void* x, int64_t ldx,
+                           int dtype, int64_t tokens, const void* q, const void* scales,
+                           int64_t out_features, int64_t in_features, void* dx, void* dw,
+                           void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * D. Pinned host memory and host<->device streaming.
  * ---------------------------------------------------------------------- */
 

@@ -123,6 +123,32 @@ SIGNATURES = {
         [c_void_p] * 4 + [c_int64] + _ADAM_TAIL
         + [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    # src, src_dtype, stride, rows, cols, q, scales, stream
+    "oa_quant_fp8": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    # q, scales, rows, cols, out, out_dtype, out_stride, stream
+    "oa_dequant_fp8": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p],
+    ),
+    # tokens, in_features, out_features, backward, want_dx, want_dw, want_db
+    "oa_fp8_linear_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 4),
+    # x, ldx, dtype, tokens, q, scales, bias, out_features, in_features, y, workspace,
+    # workspace_bytes, stream
+    "oa_fp8_linear_forward": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    # grad, ldg, x, ldx, dtype, tokens, q, scales, out_features, in_features, dx, dw, db,
+    # workspace, workspace_bytes, stream
+    "oa_fp8_linear_backward": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p, c_int64,
+         c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     # tokens, hidden, vocab, backward, want_dx, want_dw
     "oa_linear_ce_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int] * 3),
     # x, ldx, w, ldw, dtype, target, tokens, hidden, vocab, ignore_index, reduction,

@@ -1,0 +1,732 @@
+// 8-bit floating-point weights (e4m3 codes, one e8m0 scale per 128 x 128 block) and the
+// linear layer on them.
+//
+// A scale is the smallest power of two that brings the largest magnitude of its block
+// to 448 or less, so that scaling is exact and a code is one rounding of its element;
+// the matrix instruction of gfx950 applies such scales by itself.  Elements that are
+// not finite take no part in the scale and become NaN.
+//
+//   y  = xq wq^T     xq: blocks of 1 x 128 along the inputs      (T x K) (N x K)^T
+//   dx = gq wq       gq: blocks of 1 x 128 along the outputs     (T x N) (N x K)
+//   dw = gt^T xt     gt, xt: blocks of 128 x 1 along the tokens  (T x N)^T (T x K)
+//
+// Products accumulate in fp32 and are rounded once, to the type of x.
+
+#include <math.h>
+
+#include "oa_gemm.hpp"
+
+#pragma clang fp contract(off)
+
+namespace oa {
+namespace {
+
+using namespace gemm;
+
+constexpr int kBlock = 128;
+constexpr int kThreads = 256;  // 16 x 16 lanes, each 8 rows x 8 columns of a block
+constexpr int kPatch = 8;
+
+int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t blocks_of(int64_t v) { return (v + kBlock - 1) / kBlock; }
+
+template <int DT>
+__device__ __forceinline__ float load1(const void* base, int64_t i) {
+  if (DT == OA_F32) return static_cast<const float*>(base)[i];
+  const uint16_t h = static_cast<const uint16_t*>(base)[i];
+  return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* base, int64_t i, float (&x)[8]) {
+  if (DT == OA_F32) {
+    const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i);
+    const f32x4 a = p[0], b = p[1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = a[k];
+      x[4 + k] = b[k];
+    }
+  } else {
+    const u16x8 w = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(base) + i);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = DT == OA_BF16 ? bf16_bits_to_f32(w[k])
+                           : (float)__builtin_bit_cast(_Float16, (unsigned short)w[k]);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if (DT == OA_BF16) return f32x2_to_bf16x2_bits(a, b);
+  const _Float16 lo = (_Float16)a, hi = (_Float16)b;
+  return (uint32_t)__builtin_bit_cast(uint16_t, lo) |
+         ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+}
+
+template <int DT>
+__device__ __forceinline__ void store1(void* base, int64_t i, float v) {
+  if (DT == OA_F32) static_cast<float*>(base)[i] = v;
+  else static_cast<uint16_t*>(base)[i] = (uint16_t)pack16<DT>(v, 0.0f);
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(void* base, int64_t i, f32x4 v) {
+  if (DT == OA_F32) *reinterpret_cast<f32x4*>(static_cast<float*>(base) + i) = v;
+  else
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(base) + i) =
+        u32x2{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3])};
+}
+
+// e8m0 byte of a set whose largest finite magnitude is m: 448 = 1.75 * 2^8, so the
+// exponent of m, one more if its mantissa is over 1.75, less 8; at least 2^-126, and 1
+// for a set of zeros.
+__device__ __forceinline__ uint32_t scale_of(float m) {
+  const uint32_t u = __float_as_uint(m);
+  const int b = (int)((u + 0x1FFFFFu) >> 23) - 8;
+  return u == 0 ? 127u : (uint32_t)(b < 1 ? 1 : b);
+}
+// 1 / scale, exactly
+__device__ __forceinline__ float down_of(uint32_t scale) {
+  return __uint_as_float((254u - scale) << 23);
+}
+__device__ __forceinline__ float scale_value(uint32_t b) {
+  return __uint_as_float(b == 0 ? 0x00400000u : b == 255 ? 0x7FC00000u : b << 23);
+}
+
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+// One lane's 8 x 8 patch of a source: rows r0 .. r0+7, columns c0 .. c0+7; what lies
+// outside reads as zero, infinities as NaN.  `vec`: rows are 16-byte aligned and a
+// multiple of 8 columns long.
+template <int DT>
+__device__ __forceinline__ void load_patch(const void* src, int64_t stride, int64_t rows,
+                                           int64_t cols, int64_t r0, int64_t c0, bool vec,
+                                           float (&v)[kPatch][kPatch]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kPatch; ++p) {
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) v[p][j] = 0.0f;
+    if (r0 + p >= rows) continue;
+    if (vec) {
+      if (c0 < cols) load8<DT>(src, (r0 + p) * stride + c0, v[p]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j)
+        if (c0 + j < cols) v[p][j] = load1<DT>(src, (r0 + p) * stride + c0 + j);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kPatch; ++p)
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) top = fmaxf(top, fabsf(v[p][j]));
+  if (top == INFINITY) {
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p)
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j)
+        if (fabsf(v[p][j]) == INFINITY) v[p][j] = NAN;
+  }
+}
+
+// -------------------------------------------------------------- weight codec
+
+// One workgroup per 128 x 128 block: one read of the source, one write of the codes.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_encode_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
+                  int64_t blocks_c, bool vec, uint8_t* __restrict__ q,
+                  uint8_t* __restrict__ scales) {
+  __shared__ float tops[kThreads / kWave];
+  const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+  const int64_t r0 = br * kBlock + threadIdx.x / 16 * kPatch;
+  const int64_t c0 = bc * kBlock + threadIdx.x % 16 * kPatch;
+  float v[kPatch][kPatch];
+  load_patch<DT>(src, stride, rows, cols, r0, c0, vec, v);
+  float top = 0.0f;
+#pragma unroll
+  for (int p = 0; p < kPatch; ++p)
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) top = fmaxf(top, fabsf(v[p][j]));
+  top = wave_max(top);
+  if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; ++w) top = fmaxf(top, tops[w]);
+  const uint32_t s = scale_of(top);
+  const float down = down_of(s);
+  if (threadIdx.x == 0) scales[blockIdx.x] = (uint8_t)s;
+#pragma unroll
+  for (int p = 0; p < kPatch; ++p) {
+    if (r0 + p >= rows || c0 >= cols) continue;  // cols is a multiple of 16
+    float* x = v[p];
+    *reinterpret_cast<u32x2*>(q + (r0 + p) * cols + c0) =
+        u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
+              encode4(x[4] * down, x[5] * down, x[6] * down, x[7] * down)};
+  }
+}
+
+__device__ __forceinline__ void decode4(uint32_t w, float s, float* x) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  x[0] = a[0] * s;
+  x[1] = a[1] * s;
+  x[2] = b[0] * s;
+  x[3] = b[1] * s;
+}
+
+// 16 codes per lane (cols is a multiple of 16: one row, one block).
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_decode_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, int64_t rows,
+                  int64_t cols, int64_t blocks_c, void* __restrict__ out, int64_t out_stride,
+                  bool vec) {
+  const int64_t per_row = cols / 16;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= rows * per_row) return;
+  const int64_t r = i / per_row, c = i % per_row * 16;
+  const float s = scale_value(scales[r / kBlock * blocks_c + c / kBlock]);
+  const u32x4 w = *reinterpret_cast<const u32x4*>(q + r * cols + c);
+  float x[16];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) decode4(w[k], s, x + 4 * k);
+  const int64_t o = r * out_stride + c;
+  if (vec) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      store4<DT>(out, o + 4 * k, f32x4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]});
+  } else {
+    for (int k = 0; k < 16; ++k) store1<DT>(out, o + k, x[k]);
+  }
+}
+
+// Codes [rows][cols] -> [cols][ld_out], zeros for rows up to ld_out.
+__global__ void __launch_bounds__(kThreads)
+fp8_transpose_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int64_t blocks_c,
+                     uint8_t* __restrict__ out, int64_t ld_out) {
+  __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];  // [column][row]
+  const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+  const int r = threadIdx.x / 16 * kPatch, c = threadIdx.x % 16 * kPatch;
+  const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
+  u32x2 w[kPatch];
+#pragma unroll
+  for (int p = 0; p < kPatch; ++p)
+    w[p] = r0 + p < rows && c0 < cols ? *reinterpret_cast<const u32x2*>(q + (r0 + p) * cols + c0)
+                                      : u32x2{0u, 0u};
+#pragma unroll
+  for (int j = 0; j < kPatch; ++j) {
+    u8x8 o;
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p) o[p] = (uint8_t)(w[p][j / 4] >> (8 * (j % 4)));
+    *reinterpret_cast<u8x8*>(&tile[c + j][r]) = o;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = threadIdx.x + kThreads * k, col = i / 8, piece = i % 8 * 16;
+    if (bc * kBlock + col < cols)
+      *reinterpret_cast<u32x4*>(out + (bc * kBlock + col) * ld_out + br * kBlock + piece) =
+          *reinterpret_cast<const u32x4*>(&tile[col][piece]);
+  }
+}
+
+// ----------------------------------------------------------- operand encoder
+
+// A matrix [rows][cols] as operands of the products, in one read of it:
+struct Encoded {
+  uint8_t* q;        // codes [rows][ld], blocks of 1 x 128 along the columns
+  uint8_t* scales;   // packed, rows x column blocks
+  int64_t ld, scale_stride;
+  uint8_t* qt;       // codes [cols][ld_t], blocks of 128 x 1 along the rows
+  uint8_t* scales_t; // packed, cols x row blocks
+  int64_t ld_t, scale_stride_t;
+  float* sums;       // [row block][cols]: sums over 128 rows
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_operand_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
+                   int64_t blocks_c, bool vec, const Encoded e) {
+  __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];  // [column][row]
+  __shared__ float part[16][kBlock + 4];
+  __shared__ uint32_t shared_scale[kBlock];
+  const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+  const int rg = threadIdx.x / 16, cg = threadIdx.x % 16;
+  const int r = rg * kPatch, c = cg * kPatch;
+  const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
+  float v[kPatch][kPatch];
+  load_patch<DT>(src, stride, rows, cols, r0, c0, vec, v);
+
+  if (e.q) {
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p) {
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j) top = fmaxf(top, fabsf(v[p][j]));
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      const uint32_t s = scale_of(top);
+      const float down = down_of(s);
+      if (r0 + p < rows) {
+        const float* x = v[p];
+        *reinterpret_cast<u32x2*>(e.q + (r0 + p) * e.ld + c0) =
+            u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
+                  encode4(x[4] * down, x[5] * down, x[6] * down, x[7] * down)};
+        if (cg == 0) e.scales[packed_scale_at(r0 + p, bc, e.scale_stride)] = (uint8_t)s;
+      }
+    }
+  }
+  if (e.sums) {
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) {
+      float s = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kPatch; ++p) s += v[p][j];
+      part[rg][c + j] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBlock && bc * kBlock + threadIdx.x < cols) {
+      float s = 0.0f;
+      for (int g = 0; g < 16; ++g) s += part[g][threadIdx.x];
+      e.sums[br * cols + bc * kBlock + threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
+  if (!e.qt) return;
+#pragma unroll
+  for (int j = 0; j < kPatch; ++j) {
+    float top = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p) top = fmaxf(top, fabsf(v[p][j]));
+    part[rg][c + j] = top;
+  }
+  __syncthreads();
+  if (threadIdx.x < kBlock) {
+    float top = 0.0f;
+    for (int g = 0; g < 16; ++g) top = fmaxf(top, part[g][threadIdx.x]);
+    const uint32_t s = scale_of(top);
+    shared_scale[threadIdx.x] = s;
+    const int64_t col = bc * kBlock + threadIdx.x;
+    if (col < cols) e.scales_t[packed_scale_at(col, br, e.scale_stride_t)] = (uint8_t)s;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPatch; ++j) {
+    const float d = down_of(shared_scale[c + j]);
+    *reinterpret_cast<u32x2*>(&tile[c + j][r]) =
+        u32x2{encode4(v[0][j] * d, v[1][j] * d, v[2][j] * d, v[3][j] * d),
+              encode4(v[4][j] * d, v[5][j] * d, v[6][j] * d, v[7][j] * d)};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = threadIdx.x + kThreads * k, col = i / 8, piece = i % 8 * 16;
+    if (bc * kBlock + col < cols)
+      *reinterpret_cast<u32x4*>(e.qt + (bc * kBlock + col) * e.ld_t + br * kBlock + piece) =
+          *reinterpret_cast<const u32x4*>(&tile[col][piece]);
+  }
+}
+
+// Column sums: the row blocks' sums in order.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_column_sum_kernel(const float* __restrict__ sums, int64_t blocks_r, int64_t cols,
+                      void* __restrict__ out) {
+  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.0f;
+  for (int64_t b = 0; b < blocks_r; ++b) s += sums[b * cols + c];
+  store1<DT>(out, c, s);
+}
+
+// ------------------------------------------------------------------ products
+
+template <int DT>
+struct StoreEpilogue {
+  void* out;
+  int64_t rows, cols;  // p, q
+  const void* bias;    // by q, or NULL
+  bool vec;            // four columns can be stored together
+
+  template <class Tl>
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+                                             uint8_t*) const {
+#pragma unroll
+    for (int a = 0; a < Tl::QT; ++a) {
+      const int64_t q = row_q + t.q0() + 16 * a;
+      if (q >= cols) continue;
+      f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (q + i < cols) add[i] = load1<DT>(bias, q + i);
+#pragma unroll
+      for (int b = 0; b < Tl::PT; ++b) {
+        const int64_t p = row_p + t.p0() + 16 * b;
+        if (p >= rows) continue;
+        const f32x4 v = t.acc[a][b] + add;
+        if (vec) store4<DT>(out, p * cols + q, v);
+        else
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (q + i < cols) store1<DT>(out, p * cols + q + i, v[i]);
+      }
+    }
+  }
+};
+
+// One slice of a product split along k: fp32, [slice][row][cols].
+struct SliceEpilogue {
+  float* out;
+  int64_t rows, cols;
+  bool vec;
+
+  template <class Tl>
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq,
+                                             int slice, uint8_t* lds) const {
+    StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr, vec};
+    e(t, row_q, row_p, tq, 0, lds);
+  }
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_join_kernel(const float* __restrict__ part, int slices, int64_t count, int64_t cols,
+                const void* __restrict__ bias, void* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= count) return;
+  float v = part[i];
+  for (int s = 1; s < slices; ++s) v += part[s * count + i];
+  if (bias) v += load1<DT>(bias, i % cols);
+  store1<DT>(out, i, v);
+}
+
+struct Carver {
+  uint8_t* base;
+  size_t used = 0;
+  template <class P>
+  P* take(int64_t count) {
+    P* p = reinterpret_cast<P*>(base ? base + used : nullptr);
+    used += (size_t)up_to(count * (int64_t)sizeof(P), 256);
+    return p;
+  }
+};
+
+// A product's rows and columns, its output and the partial sums of its slices.
+struct Output {
+  int64_t rows, cols;
+  int slices;
+  float* part;
+  Output() : rows(0), cols(0), slices(1), part(nullptr) {}
+  Output(int64_t rows_, int64_t cols_, int64_t k_bytes, Carver& c) : rows(rows_), cols(cols_) {
+    slices = slices_for(cols, rows, k_bytes);
+    part = slices > 1 ? c.take<float>(slices * rows * cols) : nullptr;
+  }
+};
+
+template <int DT>
+int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hipStream_t s) {
+  const bool vec = o.cols % 4 == 0 && aligned_to(out, 16);
+  if (o.slices == 1) {
+    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias, vec};
+    return large_tiles_fill(o.cols, o.rows)
+               ? launch_tiles<Large<E4m3>, StoreEpilogue<DT>>(pr, 1, e, s)
+               : launch_tiles<Small<E4m3>, StoreEpilogue<DT>>(pr, 1, e, s);
+  }
+  const SliceEpilogue e{o.part, o.rows, o.cols, o.cols % 4 == 0};
+  int rc = launch_tiles<Small<E4m3>, SliceEpilogue>(pr, o.slices, e, s);
+  if (rc) return rc;
+  const int64_t count = o.rows * o.cols;
+  hipLaunchKernelGGL(fp8_join_kernel<DT>, dim3((unsigned)((count + kThreads - 1) / kThreads)),
+                     dim3(kThreads), 0, s, o.part, o.slices, count, o.cols, bias, out);
+  return launch_status();
+}
+
+struct Source {
+  const void* base;
+  int64_t stride, rows, cols;
+};
+
+bool vector_rows(const Source& m, int dtype) {
+  const int64_t per = dtype == OA_F32 ? 4 : 8;
+  return m.cols % 8 == 0 && m.stride % per == 0 && aligned_to(m.base, 16);
+}
+
+template <int DT>
+int encode_operand(const Source& m, const Encoded& e, hipStream_t s) {
+  const int64_t bc = blocks_of(m.cols), br = blocks_of(m.rows);
+  hipLaunchKernelGGL(fp8_operand_kernel<DT>, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s,
+                     m.base, m.stride, m.rows, m.cols, bc, vector_rows(m, DT), e);
+  return launch_status();
+}
+
+struct Layer {
+  const uint8_t *q, *scales;
+  int64_t out_f, in_f;
+};
+
+struct ForwardPlan {
+  Encoded x{};
+  Output y;
+  size_t bytes;
+  ForwardPlan(int64_t tokens, int64_t in_f, int64_t out_f, void* ws) {
+    Carver c{static_cast<uint8_t*>(ws)};
+    x.ld = up_to(in_f, kBlock);
+    x.scale_stride = up_to(tokens, 256);
+    x.q = c.take<uint8_t>(tokens * x.ld);
+    x.scales = c.take<uint8_t>(blocks_of(in_f) * x.scale_stride);
+    y = Output(tokens, out_f, in_f, c);
+    bytes = c.used;
+  }
+};
+
+template <int DT>
+int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws, hipStream_t s) {
+  const ForwardPlan plan(x.rows, w.in_f, w.out_f, ws);
+  int rc = encode_operand<DT>(x, plan.x, s);
+  if (rc) return rc;
+  Problem pr{};
+  pr.q = Operand{w.q, w.in_f, w.out_f};
+  pr.p = Operand{plan.x.q, plan.x.ld, x.rows};
+  pr.sq = Scales{w.scales, 1, blocks_of(w.in_f), blocks_of(w.out_f), false};
+  pr.sp = Scales{plan.x.scales, plan.x.scale_stride, 0, 0, true};
+  pr.k_bytes = (int)w.in_f;
+  return multiply<DT>(pr, plan.y, bias, y, s);
+}
+
+struct BackwardPlan {
+  Encoded g{}, x{};
+  uint8_t* wt = nullptr;
+  Output dx, dw;
+  size_t bytes;
+  BackwardPlan(int64_t tokens, int64_t in_f, int64_t out_f, bool want_dx, bool want_dw,
+               bool want_db, void* ws) {
+    Carver c{static_cast<uint8_t*>(ws)};
+    const int64_t padded_t = up_to(tokens, kBlock), padded_n = up_to(out_f, kBlock);
+    if (want_dx) {
+      g.ld = padded_n;
+      g.scale_stride = up_to(tokens, 256);
+      g.q = c.take<uint8_t>(tokens * g.ld);
+      g.scales = c.take<uint8_t>(blocks_of(out_f) * g.scale_stride);
+      wt = c.take<uint8_t>(in_f * padded_n);
+      dx = Output(tokens, in_f, padded_n, c);
+    }
+    if (want_dw) {
+      g.ld_t = x.ld_t = padded_t;
+      g.scale_stride_t = up_to(out_f, 256);
+      x.scale_stride_t = up_to(in_f, 256);
+      g.qt = c.take<uint8_t>(out_f * padded_t);
+      g.scales_t = c.take<uint8_t>(blocks_of(tokens) * g.scale_stride_t);
+      x.qt = c.take<uint8_t>(in_f * padded_t);
+      x.scales_t = c.take<uint8_t>(blocks_of(tokens) * x.scale_stride_t);
+      dw = Output(out_f, in_f, padded_t, c);
+    }
+    if (want_db) g.sums = c.take<float>(blocks_of(tokens) * out_f);
+    bytes = c.used;
+  }
+};
+
+template <int DT>
+int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* dw, void* db,
+             void* ws, hipStream_t s) {
+  const BackwardPlan plan(g.rows, w.in_f, w.out_f, dx != nullptr, dw != nullptr, db != nullptr, ws);
+  int rc = encode_operand<DT>(g, plan.g, s);
+  if (rc) return rc;
+  if (dx) {
+    const int64_t bc = blocks_of(w.in_f), br = blocks_of(w.out_f);
+    hipLaunchKernelGGL(fp8_transpose_kernel, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s, w.q,
+                       w.out_f, w.in_f, bc, plan.wt, plan.g.ld);
+    rc = launch_status();
+    if (rc) return rc;
+    Problem pr{};
+    pr.q = Operand{plan.wt, plan.g.ld, w.in_f};
+    pr.p = Operand{plan.g.q, plan.g.ld, g.rows};
+    pr.sq = Scales{w.scales, bc, 1, bc, false};
+    pr.sp = Scales{plan.g.scales, plan.g.scale_stride, 0, 0, true};
+    pr.k_bytes = (int)plan.g.ld;
+    rc = multiply<DT>(pr, plan.dx, nullptr, dx, s);
+    if (rc) return rc;
+  }
+  if (dw) {
+    rc = encode_operand<DT>(x, plan.x, s);
+    if (rc) return rc;
+    Problem pr{};
+    pr.q = Operand{plan.x.qt, plan.x.ld_t, w.in_f};
+    pr.p = Operand{plan.g.qt, plan.g.ld_t, w.out_f};
+    pr.sq = Scales{plan.x.scales_t, plan.x.scale_stride_t, 0, 0, true};
+    pr.sp = Scales{plan.g.scales_t, plan.g.scale_stride_t, 0, 0, true};
+    pr.k_bytes = (int)plan.x.ld_t;
+    rc = multiply<DT>(pr, plan.dw, nullptr, dw, s);
+    if (rc) return rc;
+  }
+  if (db) {
+    hipLaunchKernelGGL(fp8_column_sum_kernel<DT>,
+                       dim3((unsigned)((w.out_f + kThreads - 1) / kThreads)), dim3(kThreads), 0, s,
+                       plan.g.sums, blocks_of(g.rows), w.out_f, db);
+    rc = launch_status();
+  }
+  return rc;
+}
+
+bool known(int dtype) { return dtype == OA_F32 || dtype == OA_BF16 || dtype == OA_F16; }
+uintptr_t size_of(int dtype) { return dtype == OA_F32 ? 4 : 2; }
+
+constexpr int64_t kMostRows = (int64_t)1 << 22;  // of an operand; also its longest row
+
+int check_codec(const void* q, const void* scales, int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0 || cols % 16 || (rows > 0 && cols > 0 && (!q || !scales)))
+    return OA_EINVAL;
+  if (!aligned_to(q, 16)) return OA_EALIGN;
+  if (blocks_of(rows) * blocks_of(cols) > 0x7FFFFFFF ||
+      (cols > 0 && rows > ((int64_t)0x7FFFFFFF * kThreads) / (cols / 16)))
+    return OA_ERANGE;
+  return 0;
+}
+
+int check_layer(const Layer& w, int64_t tokens, int dtype) {
+  if (!known(dtype) || tokens <= 0 || w.out_f <= 0 || w.in_f <= 0 || w.in_f % 16 || !w.q ||
+      !w.scales)
+    return OA_EINVAL;
+  if (!aligned_to(w.q, 16)) return OA_EALIGN;
+  if (tokens > kMostRows || w.out_f > kMostRows || w.in_f > kMostRows) return OA_ERANGE;
+  return 0;
+}
+
+int check_source(const Source& m, int dtype) {
+  if (!m.base || (m.rows > 1 && m.stride < m.cols)) return OA_EINVAL;
+  return aligned_to(m.base, size_of(dtype)) ? 0 : OA_EALIGN;
+}
+
+}  // namespace
+}  // namespace oa
+
+using namespace oa;
+
+extern "C" int oa_quant_fp8(const void* src, int src_dtype, int64_t src_row_stride, int64_t rows,
+                            int64_t cols, void* q, void* scales, void* stream) {
+  int rc = check_codec(q, scales, rows, cols);
+  if (rc) return rc;
+  if (!known(src_dtype) || src_row_stride < 0) return OA_EINVAL;
+  if (rows == 0 || cols == 0) return 0;
+  const Source m{src, src_row_stride, rows, cols};
+  rc = check_source(m, src_dtype);
+  if (rc) return rc;
+  const bool vec = vector_rows(m, src_dtype);
+  const int64_t bc = blocks_of(cols);
+  const dim3 grid((unsigned)(bc * blocks_of(rows)));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t *qb = static_cast<uint8_t*>(q), *sb = static_cast<uint8_t*>(scales);
+  switch (src_dtype) {
+    case OA_F32:
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_F32>, grid, dim3(kThreads), 0, s, src,
+                         src_row_stride, rows, cols, bc, vec, qb, sb);
+      break;
+    case OA_BF16:
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_BF16>, grid, dim3(kThreads), 0, s, src,
+                         src_row_stride, rows, cols, bc, vec, qb, sb);
+      break;
+    default:
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_F16>, grid, dim3(kThreads), 0, s, src,
+                         src_row_stride, rows, cols, bc, vec, qb, sb);
+  }
+  return launch_status();
+}
+
+extern "C" int oa_dequant_fp8(const void* q, const void* scales, int64_t rows, int64_t cols,
+                              void* out, int out_dtype, int64_t out_row_stride, void* stream) {
+  int rc = check_codec(q, scales, rows, cols);
+  if (rc) return rc;
+  if (!known(out_dtype) || (rows > 1 && out_row_stride < cols)) return OA_EINVAL;
+  if (rows == 0 || cols == 0) return 0;
+  if (!out) return OA_EINVAL;
+  if (!aligned_to(out, size_of(out_dtype))) return OA_EALIGN;
+  const bool vec = out_row_stride % 8 == 0 && aligned_to(out, 16);
+  const int64_t bc = blocks_of(cols), lanes = rows * (cols / 16);
+  const dim3 grid((unsigned)((lanes + kThreads - 1) / kThreads));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const uint8_t *qb = static_cast<const uint8_t*>(q), *sb = static_cast<const uint8_t*>(scales);
+  switch (out_dtype) {
+    case OA_F32:
+      hipLaunchKernelGGL(fp8_decode_kernel<OA_F32>, grid, dim3(kThreads), 0, s, qb, sb, rows, cols,
+                         bc, out, out_row_stride, vec);
+      break;
+    case OA_BF16:
+      hipLaunchKernelGGL(fp8_decode_kernel<OA_BF16>, grid, dim3(kThreads), 0, s, qb, sb, rows,
+                         cols, bc, out, out_row_stride, vec);
+      break;
+    default:
+      hipLaunchKernelGGL(fp8_decode_kernel<OA_F16>, grid, dim3(kThreads), 0, s, qb, sb, rows, cols,
+                         bc, out, out_row_stride, vec);
+  }
+  return launch_status();
+}
+
+extern "C" size_t oa_fp8_linear_workspace_bytes(int64_t tokens, int64_t in_features,
+                                                int64_t out_features, int backward, int want_dx,
+                                                int want_dw, int want_db) {
+  if (tokens <= 0 || in_features <= 0 || out_features <= 0) return 0;
+  if (!backward) return ForwardPlan(tokens, in_features, out_features, nullptr).bytes;
+  return BackwardPlan(tokens, in_features, out_features, want_dx != 0, want_dw != 0, want_db != 0,
+                      nullptr)
+      .bytes;
+}
+
+extern "C" int oa_fp8_linear_forward(const void* x, int64_t ldx, int dtype, int64_t tokens,
+                                     const void* q, const void* scales, const void* bias,
+                                     int64_t out_features, int64_t in_features, void* y,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  const Layer w{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales), out_features,
+                in_features};
+  int rc = check_layer(w, tokens, dtype);
+  if (rc) return rc;
+  const Source m{x, ldx, tokens, in_features};
+  rc = check_source(m, dtype);
+  if (rc) return rc;
+  if (!y || !workspace ||
+      workspace_bytes < oa_fp8_linear_workspace_bytes(tokens, in_features, out_features, 0, 0, 0, 0))
+    return OA_EINVAL;
+  if (!aligned_to(y, size_of(dtype)) || !aligned_to(bias, size_of(dtype)) ||
+      !aligned_to(workspace, 256))
+    return OA_EALIGN;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case OA_F32: return forward<OA_F32>(m, w, bias, y, workspace, s);
+    case OA_BF16: return forward<OA_BF16>(m, w, bias, y, workspace, s);
+    default: return forward<OA_F16>(m, w, bias, y, workspace, s);
+  }
+}
+
+extern "C" int oa_fp8_linear_backward(const void* grad, int64_t ldg, const void* x, int64_t ldx,
+                                      int dtype, int64_t tokens, const void* q,
+                                      const void* scales, int64_t out_features,
+                                      int64_t in_features, void* dx, void* dw, void* db,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  const Layer w{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scales), out_features,
+                in_features};
+  int rc = check_layer(w, tokens, dtype);
+  if (rc) return rc;
+  const Source mg{grad, ldg, tokens, out_features}, mx{x, ldx, tokens, in_features};
+  rc = check_source(mg, dtype);
+  if (rc) return rc;
+  if (dw) {
+    rc = check_source(mx, dtype);
+    if (rc) return rc;
+  }
+  if ((!dx && !dw && !db) || !workspace ||
+      workspace_bytes < oa_fp8_linear_workspace_bytes(tokens, in_features, out_features, 1,
+                                                      dx != nullptr, dw != nullptr, db != nullptr))
+    return OA_EINVAL;
+  if (!aligned_to(dx, size_of(dtype)) || !aligned_to(dw, size_of(dtype)) ||
+      !aligned_to(db, size_of(dtype)) || !aligned_to(workspace, 256))
+    return OA_EALIGN;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case OA_F32: return backward<OA_F32>(mg, mx, w, dx, dw, db, workspace, s);
+    case OA_BF16: return backward<OA_BF16>(mg, mx, w, dx, dw, db, workspace, s);
+    default: return backward<OA_F16>(mg, mx, w, dx, dw, db, workspace, s);
+  }
+}

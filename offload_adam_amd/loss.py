@@ -124,7 +124,9 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     on anything but the arguments: no atomics, one order of summation.
 
     Works on ``x``'s device and the current stream, synchronises nothing, and may be
-    captured into a graph (with the backward pass inside the same capture).
+    captured into a graph, with the backward pass inside the same capture and no eager
+    graph of the same leaves alive (torch ends the process when such a leaf's gradient
+    is accumulated during a capture).
     """
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError("x and weight must be tensors")

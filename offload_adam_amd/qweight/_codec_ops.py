@@ -3,7 +3,7 @@ fresh (or given) tensor.  GPU tensors only; every function enqueues on the
 current stream of the tensor's device and returns without synchronising.
 """
 
-from ctypes import c_int, c_int64
+from ctypes import c_int, c_int64, c_size_t
 
 import torch
 
@@ -167,3 +167,79 @@ def dequantize_nvfp4(packed, block_scale_fp8, global_scale, in_f, out_dtype):
           _lib.ptr(global_scale), c_int64(rows), c_int64(in_f), _lib.ptr(out),
           c_int(_lib.dtype_code(out_dtype)), c_int64(max(in_f, 1)))
     return out
+
+
+# --------------------------------------------------------------------- FP8
+
+FP8_BLOCK = 128
+
+
+def _fp8_payload(codes, scale):
+    rows, cols = codes.shape
+    _payload(codes, "weight", torch.float8_e4m3fn, (rows, cols))
+    _payload(scale, "block_scale", torch.float8_e8m0fnu,
+             (-(-rows // FP8_BLOCK), -(-cols // FP8_BLOCK)))
+    if scale.device != codes.device:
+        raise ValueError("weight and block_scale must be on the same GPU")
+    return rows, cols
+
+
+def quantize_fp8_into(src, codes, scale):
+    src, stride = _rows_view(src)
+    rows, cols = _fp8_payload(codes, scale)
+    if tuple(src.shape) != (rows, cols) or src.device != codes.device:
+        raise ValueError(f"cannot encode {tuple(src.shape)} on {src.device} into a "
+                         f"{rows} x {cols} weight on {codes.device}")
+    _call("oa_quant_fp8", src.device, _lib.ptr(src), c_int(_lib.dtype_code(src.dtype)),
+          c_int64(stride), c_int64(rows), c_int64(cols), _lib.ptr(codes), _lib.ptr(scale))
+    mark_written(codes, scale)
+
+
+def dequantize_fp8(codes, scale, out_dtype):
+    rows, cols = _fp8_payload(codes, scale)
+    out = torch.empty((rows, cols), dtype=out_dtype, device=codes.device)
+    _call("oa_dequant_fp8", codes.device, _lib.ptr(codes), _lib.ptr(scale), c_int64(rows),
+          c_int64(cols), _lib.ptr(out), c_int(_lib.dtype_code(out_dtype)), c_int64(max(cols, 1)))
+    return out
+
+
+def _fp8_workspace(device, *sizes):
+    nbytes = _lib.load().oa_fp8_linear_workspace_bytes(*[c_int64(v) for v in sizes[:3]],
+                                                       *[c_int(v) for v in sizes[3:]])
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def fp8_linear_forward(x, codes, scale, bias):
+    """x (T, in) -> (T, out) in x's dtype."""
+    x, ldx = _rows_view(x)
+    out_f, in_f = _fp8_payload(codes, scale)
+    dt = c_int(_lib.dtype_code(x.dtype))
+    tokens, dev = x.shape[0], x.device
+    y = torch.empty((tokens, out_f), dtype=x.dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    ws = _fp8_workspace(dev, tokens, in_f, out_f, 0, 0, 0, 0)
+    _call("oa_fp8_linear_forward", dev, _lib.ptr(x), c_int64(ldx), dt, c_int64(tokens),
+          _lib.ptr(codes), _lib.ptr(scale), _lib.ptr(bias), c_int64(out_f), c_int64(in_f),
+          _lib.ptr(y), _lib.ptr(ws), c_size_t(ws.numel()))
+    return y
+
+
+def fp8_linear_backward(grad, x, codes, scale, want_dx, want_dw, want_db):
+    """grad (T, out), x (T, in) -> (dx, dw, db) in x's dtype, None where not wanted."""
+    grad, ldg = _rows_view(grad)
+    x, ldx = _rows_view(x)
+    out_f, in_f = _fp8_payload(codes, scale)
+    dt = c_int(_lib.dtype_code(x.dtype))
+    tokens, dev = x.shape[0], x.device
+    make = torch.empty if tokens and out_f else torch.zeros
+    dx = make((tokens, in_f), dtype=x.dtype, device=dev) if want_dx else None
+    dw = make((out_f, in_f), dtype=x.dtype, device=dev) if want_dw else None
+    db = make((out_f,), dtype=x.dtype, device=dev) if want_db else None
+    if tokens and out_f and (want_dx or want_dw or want_db):
+        ws = _fp8_workspace(dev, tokens, in_f, out_f, 1, int(want_dx), int(want_dw), int(want_db))
+        _call("oa_fp8_linear_backward", dev, _lib.ptr(grad), c_int64(ldg), _lib.ptr(x),
+              c_int64(ldx), dt, c_int64(tokens), _lib.ptr(codes), _lib.ptr(scale),
+              c_int64(out_f), c_int64(in_f), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
+              _lib.ptr(ws), c_size_t(ws.numel()))
+    return dx, dw, db

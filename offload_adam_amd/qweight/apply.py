@@ -46,8 +46,8 @@ class _PlainTensorHooks:
                 unexpected_keys, error_msgs):
         suffixes = self.weight_cls.canonical_key_suffixes()
         found = {s: state_dict.pop(prefix + s) for s in suffixes if prefix + s in state_dict}
-        # a float "weight" is an ordinary checkpoint: put it back, copy_ re-quantises
-        if "weight" in found and found["weight"].dtype is not torch.uint8:
+        # a "weight" that is not codes is an ordinary checkpoint: put it back, copy_ re-quantises
+        if "weight" in found and found["weight"].dtype not in (torch.uint8, torch.float8_e4m3fn):
             state_dict[prefix + "weight"] = found.pop("weight")
         if not found:
             return

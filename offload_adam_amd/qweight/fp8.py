@@ -1,0 +1,248 @@
+"""FP8 (e4m3) QAT weight with one scale per 128 x 128 block, and the linear layer whose
+products run on 8-bit codes.
+
+Payload:
+  weight      : (out_f, in_f) float8_e4m3fn codes, in_f a multiple of 16
+  block_scale : (ceil(out_f / 128), ceil(in_f / 128)) float8_e8m0fnu - a power of two;
+                value = code * scale
+
+A scale is the smallest power of two (at least 2^-126) that brings the largest finite
+magnitude of its block to 448, the e4m3 maximum, or less; 1 for a block of zeros.
+Scaling is then exact, every code is its element rounded once (to nearest even), and
+decoding is exact; the matrix instructions of gfx950 apply such scales by themselves.
+Elements that are not finite become NaN.
+
+Unlike the package's other formats, which decode the weight and multiply in the
+activations' dtype, ``F.linear`` on this one also encodes its other operand, in blocks of
+128 along the dimension that the product sums over, and multiplies codes:
+
+  y  = enc(x) W^T + b      blocks of 128 inputs of a token
+  dx = enc(dy) W           blocks of 128 outputs of a token
+  dw = enc(dy)^T enc(x)    blocks of 128 tokens of an output / input
+  db = sum of dy           not encoded
+
+with fp32 sums and one rounding to the dtype of ``x``.  The reference has no counterpart
+(its formats are weight-only, src/offload_adam/qweight/).
+"""
+
+from typing import Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _codec_ops
+from .base import QWeightBase
+
+FP8_BLOCK = _codec_ops.FP8_BLOCK
+FP8_E4M3_MAX = 448.0
+_HIP_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _power_of_two(e: Tensor) -> Tensor:
+    """2^e for integer e in [-126, 127], by its bits (exp2 may be an ulp off)."""
+    return ((e + 127) << 23).to(torch.int32).view(torch.float32)
+
+
+def _encode_blocks(x: Tensor, rows: int, cols: int) -> Tuple[Tensor, Tensor]:
+    """float (R, C) -> (codes (R, C), exponents (R / rows, C / cols)): torch arithmetic."""
+    r, c = x.shape
+    x = torch.nn.functional.pad(x.float(), (0, -c % cols, 0, -r % rows))
+    b = x.reshape(x.shape[0] // rows, rows, x.shape[1] // cols, cols)
+    finite = torch.isfinite(b)
+    top = torch.where(finite, b.abs(), 0.0).amax(dim=(1, 3))
+    mantissa, e = torch.frexp(top)  # top = mantissa * 2^e, 448 = 0.875 * 2^9
+    e = torch.where(mantissa > FP8_E4M3_MAX / 512, e - 8, e - 9)
+    e = torch.where(top == 0, 0, e).clamp(min=-126)
+    b = torch.where(finite, b * _power_of_two(-e)[:, None, :, None], float("nan"))
+    codes = b.reshape(x.shape).to(torch.float8_e4m3fn)[:r, :c]
+    return codes.contiguous(), e
+
+
+def _decode_blocks(codes: Tensor, scale: Tensor, rows: int, cols: int) -> Tensor:
+    """fp32 values of codes with one scale per rows x cols block."""
+    r, c = codes.shape
+    spread = scale.float().repeat_interleave(rows, 0)[:r].repeat_interleave(cols, 1)[:, :c]
+    return codes.float() * spread
+
+
+def _held(x: Tensor, rows: int, cols: int) -> Tensor:
+    codes, e = _encode_blocks(x, rows, cols)
+    return _decode_blocks(codes, _power_of_two(e), rows, cols)
+
+
+@torch.no_grad()
+def quantize_fp8_blockwise(tensor: Tensor) -> Tuple[Tensor, Tensor]:
+    """(out_f, in_f) float -> (float8_e4m3fn codes, float8_e8m0fnu block scales)."""
+    assert tensor.ndim == 2 and tensor.shape[1] % 16 == 0
+    if tensor.is_cuda:
+        return _quantize_fp8_hip(tensor)
+    codes, e = _encode_blocks(tensor, FP8_BLOCK, FP8_BLOCK)
+    return codes, (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def dequantize_fp8_blockwise(weight: Tensor, block_scale: Tensor,
+                             dtype=torch.float32) -> Tensor:
+    """codes * scale in ``dtype``."""
+    if weight.is_cuda and dtype in _HIP_DTYPES:
+        return _codec_ops.dequantize_fp8(weight.contiguous(), block_scale.contiguous(), dtype)
+    return _decode_blocks(weight, block_scale, FP8_BLOCK, FP8_BLOCK).to(dtype)
+
+
+def _quantize_fp8_hip(tensor):
+    out_f, in_f = tensor.shape
+    dev = tensor.device
+    weight = torch.empty((out_f, in_f), dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty((-(-out_f // FP8_BLOCK), -(-in_f // FP8_BLOCK)),
+                        dtype=torch.float8_e8m0fnu, device=dev)
+    _codec_ops.quantize_fp8_into(tensor, weight, scale)
+    return weight, scale
+
+
+class _FP8Linear(torch.autograd.Function):
+    """GPU operands go to the HIP kernels; CPU operands (model surgery, host tests) take
+    the same definition in torch arithmetic."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(x, weight)
+        flat = x.reshape(-1, x.shape[-1])
+        if x.is_cuda:
+            y = _codec_ops.fp8_linear_forward(flat, weight.weight, weight.block_scale, bias)
+        else:
+            y = _held(flat, 1, FP8_BLOCK) @ weight.dequantize(torch.float32).T
+            y = (y if bias is None else y + bias.float()).to(x.dtype)
+        return y.reshape(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight = ctx.saved_tensors
+        want_dx, want_dw, want_db = ctx.needs_input_grad
+        flat = x.reshape(-1, x.shape[-1])
+        g = grad.reshape(-1, weight.shape[0])
+        if x.is_cuda:
+            dx, dw, db = _codec_ops.fp8_linear_backward(
+                g, flat, weight.weight, weight.block_scale, want_dx, want_dw, want_db)
+        else:
+            dx = dw = db = None
+            if want_dx:
+                dx = (_held(g, 1, FP8_BLOCK) @ weight.dequantize(torch.float32)).to(x.dtype)
+            if want_dw:
+                dw = (_held(g, FP8_BLOCK, 1).T @ _held(flat, FP8_BLOCK, 1)).to(x.dtype)
+            if want_db:
+                db = g.float().sum(0).to(x.dtype)
+        return dx.reshape(x.shape) if want_dx else None, dw, db
+
+
+class FP8QWeight(QWeightBase):
+    """Outer shape (out_f, in_f) at ``outer_dtype``; ``copy_`` from a plain tensor
+    re-quantises in place."""
+
+    _PAYLOAD = ("weight", "block_scale")
+
+    @staticmethod
+    @torch._dynamo.disable
+    def __new__(cls, weight, block_scale, outer_dtype):
+        return Tensor._make_wrapper_subclass(
+            cls, tuple(weight.shape), dtype=outer_dtype, device=weight.device
+        )
+
+    @torch._dynamo.disable
+    def __init__(self, weight, block_scale, outer_dtype):
+        assert weight.dtype is torch.float8_e4m3fn and weight.ndim == 2
+        assert weight.shape[1] % 16 == 0
+        assert block_scale.dtype is torch.float8_e8m0fnu
+        assert tuple(block_scale.shape) == tuple(-(-n // FP8_BLOCK) for n in weight.shape)
+        self.weight = weight
+        self.block_scale = block_scale
+        self.outer_dtype = outer_dtype
+
+    def _meta(self):
+        return (self.outer_dtype,)
+
+    def _meta_to(self, dtype):
+        return (dtype if dtype is not None else self.outer_dtype,)
+
+    @classmethod
+    def from_float(cls, tensor: Tensor, **_):
+        weight, scale = quantize_fp8_blockwise(tensor.detach())
+        out = cls(weight, scale, tensor.dtype)
+        out.requires_grad_(tensor.requires_grad)
+        return out
+
+    @classmethod
+    def can_quantize(cls, tensor: Tensor, **_) -> bool:
+        # rows of codes have to be whole 16-byte pieces
+        return tensor.dim() == 2 and tensor.shape[1] % 16 == 0
+
+    def _requantize_(self, src: Tensor) -> None:
+        if self.weight.is_cuda:
+            src = src.detach().to(self.weight.device, non_blocking=True)
+            _codec_ops.quantize_fp8_into(src, self.weight, self.block_scale)
+        else:
+            weight, scale = quantize_fp8_blockwise(src.detach().to(self.weight.device))
+            self.weight.copy_(weight)
+            self.block_scale.copy_(scale)
+
+    def dequantize(self, dtype=None) -> Tensor:
+        return dequantize_fp8_blockwise(self.weight, self.block_scale,
+                                        self.outer_dtype if dtype is None else dtype)
+
+    # ---- serialisation: block-scaled fp8 checkpoints (codes and fp32 scales) ---
+
+    @classmethod
+    def canonical_key_suffixes(cls) -> Tuple[str, ...]:
+        return ("weight", "weight_scale_inv")
+
+    def to_plain_state_dict(self) -> dict:
+        return {"weight": self.weight, "weight_scale_inv": self.block_scale.float()}
+
+    @classmethod
+    def from_plain_state_dict(cls, plain: dict, reference=None) -> "FP8QWeight":
+        """Scales that are powers of two are taken as they are; a checkpoint with any
+        other (finite, positive) scales is encoded again from the values it stands for."""
+        if reference is None:
+            raise ValueError(
+                "FP8QWeight.from_plain_state_dict requires a reference instance to "
+                "resolve outer_dtype; the canonical state_dict carries no outer-dtype field."
+            )
+        weight, scale = plain["weight"], plain["weight_scale_inv"].float()
+        bits = scale.view(torch.int32)
+        exponent = bits >> 23  # sign and exponent field of a positive normal number
+        if bool(((bits & 0x7FFFFF) == 0).all() and ((exponent > 0) & (exponent < 255)).all()):
+            held = exponent.to(torch.uint8).view(torch.float8_e8m0fnu)
+            return cls(weight, held, reference.outer_dtype)
+        value = _decode_blocks(weight, scale, FP8_BLOCK, FP8_BLOCK)
+        return cls(*quantize_fp8_blockwise(value), reference.outer_dtype)
+
+    @classmethod
+    def build_hf_quantization_config(cls, skip_patterns=(), **_) -> dict:
+        return {
+            "quant_method": "fp8",
+            "activation_scheme": "dynamic",
+            "weight_block_size": [FP8_BLOCK, FP8_BLOCK],
+            "modules_to_not_convert": list(skip_patterns),
+        }
+
+
+@FP8QWeight.implements_torch_function(torch.nn.functional.linear)
+def _linear(func, types, args, kwargs):
+    def run(input, weight, bias=None):
+        if not isinstance(weight, FP8QWeight) or isinstance(input, FP8QWeight):
+            raise TypeError("linear: an FP8QWeight is taken as the weight only")
+        if input.dtype not in _HIP_DTYPES:
+            raise TypeError(f"linear: input must be float32, bfloat16 or float16, got {input.dtype}")
+        if input.dim() < 1 or input.shape[-1] != weight.shape[1]:
+            raise ValueError(f"linear: input {tuple(input.shape)} and weight "
+                             f"{tuple(weight.shape)} do not match")
+        if input.device != weight.device:
+            raise ValueError(f"linear: input is on {input.device}, weight on {weight.device}")
+        if bias is not None:
+            if tuple(bias.shape) != (weight.shape[0],) or bias.device != input.device:
+                raise ValueError(f"linear: bias must have shape ({weight.shape[0]},) on "
+                                 f"{input.device}, got {tuple(bias.shape)} on {bias.device}")
+            bias = bias.to(input.dtype).contiguous()
+        return _FP8Linear.apply(input, weight, bias)
+
+    return run(*args, **kwargs)
