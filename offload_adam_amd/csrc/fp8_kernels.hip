@@ -27,7 +27,6 @@ constexpr int kBlock = 128;
 constexpr int kThreads = 256;  // 16 x 16 lanes, each 8 rows x 8 columns of a block
 constexpr int kPatch = 8;
 
-int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t blocks_of(int64_t v) { return (v + kBlock - 1) / kBlock; }
 
 template <int DT>
@@ -345,36 +344,54 @@ fp8_column_sum_kernel(const float* __restrict__ sums, int64_t blocks_r, int64_t 
 
 // ------------------------------------------------------------------ products
 
+// The product, plus the bias of its columns, in the caller's type.
 template <int DT>
 struct StoreEpilogue {
   void* out;
   int64_t rows, cols;  // p, q
   const void* bias;    // by q, or NULL
-  bool vec;            // four columns can be stored together
+  bool vec;            // rows of the result are 16-byte aligned, whole octets
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
-                                             uint8_t*) const {
+                                             uint8_t* lds) const {
+    if (bias) {
 #pragma unroll
-    for (int a = 0; a < Tl::QT; ++a) {
-      const int64_t q = row_q + t.q0() + 16 * a;
-      if (q >= cols) continue;
-      f32x4 add = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (bias)
+      for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (q + i < cols) add[i] = load1<DT>(bias, q + i);
+        for (int i = 0; i < 4; ++i) {
+          const int64_t q = row_q + t.q0() + kLines * u + i;
+          const float add = q < cols ? load1<DT>(bias, q) : 0.0f;
 #pragma unroll
-      for (int b = 0; b < Tl::PT; ++b) {
-        const int64_t p = row_p + t.p0() + 16 * b;
-        if (p >= rows) continue;
-        const f32x4 v = t.acc[a][b] + add;
-        if (vec) store4<DT>(out, p * cols + q, v);
+          for (int b = 0; b < Tl::kColumns; ++b) t.acc[u][b][i] += add;
+        }
+    }
+    if constexpr (DT == OA_F32) {
+      t.rows32(lds, [&](int p, int q, f32x4 v) {
+        if (row_p + p >= rows) return;
+        float* o = static_cast<float*>(out) + (row_p + p) * cols + row_q + q;
+        if (vec && row_q + q < cols) *reinterpret_cast<f32x4*>(o) = v;
         else
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (q + i < cols) store1<DT>(out, p * cols + q + i, v[i]);
-      }
+            if (row_q + q + i < cols) o[i] = v[i];
+      });
+    } else {
+      t.rows16(
+          lds,
+          [&](int u, int b) {
+            const f32x4 v = t.quad(u, b);
+            return u32x2{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3])};
+          },
+          [&](int p, int q, u32x4 v) {
+            if (row_p + p >= rows) return;
+            uint16_t* o = static_cast<uint16_t*>(out) + (row_p + p) * cols + row_q + q;
+            if (vec && row_q + q < cols) *reinterpret_cast<u32x4*>(o) = v;
+            else
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (row_q + q + i < cols) o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+          });
     }
   }
 };
@@ -388,7 +405,7 @@ struct SliceEpilogue {
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq,
                                              int slice, uint8_t* lds) const {
-    StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr, vec};
+    const StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr, vec};
     e(t, row_q, row_p, tq, 0, lds);
   }
 };
@@ -405,44 +422,31 @@ fp8_join_kernel(const float* __restrict__ part, int slices, int64_t count, int64
   store1<DT>(out, i, v);
 }
 
-struct Carver {
-  uint8_t* base;
-  size_t used = 0;
-  template <class P>
-  P* take(int64_t count) {
-    P* p = reinterpret_cast<P*>(base ? base + used : nullptr);
-    used += (size_t)up_to(count * (int64_t)sizeof(P), 256);
-    return p;
-  }
-};
-
-// A product's rows and columns, its output and the partial sums of its slices.
+// A product's rows and columns, how it is cut, and the partial sums of its slices.
 struct Output {
-  int64_t rows, cols;
-  int slices;
-  float* part;
-  Output() : rows(0), cols(0), slices(1), part(nullptr) {}
+  int64_t rows = 0, cols = 0;
+  Cut cut{false, 1};
+  float* part = nullptr;
+  Output() {}
   Output(int64_t rows_, int64_t cols_, int64_t k_bytes, Carver& c) : rows(rows_), cols(cols_) {
-    slices = slices_for(cols, rows, k_bytes);
-    part = slices > 1 ? c.take<float>(slices * rows * cols) : nullptr;
+    cut = cut_for(cols, rows, steps_of(k_bytes), true);
+    if (cut.slices > 1) part = c.take<float>(cut.slices * rows * cols);
   }
 };
 
-template <int DT>
+template <int DT, bool Q_PACKED>
 int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hipStream_t s) {
-  const bool vec = o.cols % 4 == 0 && aligned_to(out, 16);
-  if (o.slices == 1) {
-    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias, vec};
-    return large_tiles_fill(o.cols, o.rows)
-               ? launch_tiles<Large<E4m3>, StoreEpilogue<DT>>(pr, 1, e, s)
-               : launch_tiles<Small<E4m3>, StoreEpilogue<DT>>(pr, 1, e, s);
+  typedef E4m3<Q_PACKED> T;
+  if (o.cut.slices == 1) {
+    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias, o.cols % 8 == 0 && aligned_to(out, 16)};
+    return launch_product<T, false, false>(pr, o.cut, e, s);
   }
   const SliceEpilogue e{o.part, o.rows, o.cols, o.cols % 4 == 0};
-  int rc = launch_tiles<Small<E4m3>, SliceEpilogue>(pr, o.slices, e, s);
+  int rc = launch_product<T, false, false>(pr, o.cut, e, s);
   if (rc) return rc;
   const int64_t count = o.rows * o.cols;
   hipLaunchKernelGGL(fp8_join_kernel<DT>, dim3((unsigned)((count + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, s, o.part, o.slices, count, o.cols, bias, out);
+                     dim3(kThreads), 0, s, o.part, o.cut.slices, count, o.cols, bias, out);
   return launch_status();
 }
 
@@ -490,12 +494,12 @@ int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws
   int rc = encode_operand<DT>(x, plan.x, s);
   if (rc) return rc;
   Problem pr{};
-  pr.q = Operand{w.q, w.in_f, w.out_f};
-  pr.p = Operand{plan.x.q, plan.x.ld, x.rows};
-  pr.sq = Scales{w.scales, 1, blocks_of(w.in_f), blocks_of(w.out_f), false};
-  pr.sp = Scales{plan.x.scales, plan.x.scale_stride, 0, 0, true};
+  pr.q = Operand{w.q, w.in_f, w.out_f, 0};
+  pr.p = Operand{plan.x.q, plan.x.ld, x.rows, 0};
+  pr.sq = Scales{w.scales, 1, blocks_of(w.in_f), blocks_of(w.out_f)};
+  pr.sp = Scales{plan.x.scales, plan.x.scale_stride, 0, 0};
   pr.k_bytes = (int)w.in_f;
-  return multiply<DT>(pr, plan.y, bias, y, s);
+  return multiply<DT, false>(pr, plan.y, bias, y, s);
 }
 
 struct BackwardPlan {
@@ -543,24 +547,24 @@ int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* d
     rc = launch_status();
     if (rc) return rc;
     Problem pr{};
-    pr.q = Operand{plan.wt, plan.g.ld, w.in_f};
-    pr.p = Operand{plan.g.q, plan.g.ld, g.rows};
-    pr.sq = Scales{w.scales, bc, 1, bc, false};
-    pr.sp = Scales{plan.g.scales, plan.g.scale_stride, 0, 0, true};
+    pr.q = Operand{plan.wt, plan.g.ld, w.in_f, 0};
+    pr.p = Operand{plan.g.q, plan.g.ld, g.rows, 0};
+    pr.sq = Scales{w.scales, bc, 1, bc};
+    pr.sp = Scales{plan.g.scales, plan.g.scale_stride, 0, 0};
     pr.k_bytes = (int)plan.g.ld;
-    rc = multiply<DT>(pr, plan.dx, nullptr, dx, s);
+    rc = multiply<DT, false>(pr, plan.dx, nullptr, dx, s);
     if (rc) return rc;
   }
   if (dw) {
     rc = encode_operand<DT>(x, plan.x, s);
     if (rc) return rc;
     Problem pr{};
-    pr.q = Operand{plan.x.qt, plan.x.ld_t, w.in_f};
-    pr.p = Operand{plan.g.qt, plan.g.ld_t, w.out_f};
-    pr.sq = Scales{plan.x.scales_t, plan.x.scale_stride_t, 0, 0, true};
-    pr.sp = Scales{plan.g.scales_t, plan.g.scale_stride_t, 0, 0, true};
+    pr.q = Operand{plan.x.qt, plan.x.ld_t, w.in_f, 0};
+    pr.p = Operand{plan.g.qt, plan.g.ld_t, w.out_f, 0};
+    pr.sq = Scales{plan.x.scales_t, plan.x.scale_stride_t, 0, 0};
+    pr.sp = Scales{plan.g.scales_t, plan.g.scale_stride_t, 0, 0};
     pr.k_bytes = (int)plan.x.ld_t;
-    rc = multiply<DT>(pr, plan.dw, nullptr, dw, s);
+    rc = multiply<DT, true>(pr, plan.dw, nullptr, dw, s);
     if (rc) return rc;
   }
   if (db) {

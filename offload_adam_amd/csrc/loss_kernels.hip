@@ -1,13 +1,14 @@
 // Softmax cross entropy of a linear head, z = x W^T, without ever holding z.
 //
 // Forward: the tiled product of oa_gemm.hpp with an epilogue that folds each
-// token's tile of logits into a running maximum and sum of exponentials (one pair
-// per token and tile) and picks out the target's logit; a second kernel joins the
-// pairs into lse_t = log sum_v exp z[t,v] and the losses lse_t - z[t,y_t].
+// token's tile of logits into a maximum and a sum of exponentials (one pair per token and
+// tile) and picks out the target's logit; a second kernel joins the pairs into
+// lse_t = log sum_v exp z[t,v] and the losses lse_t - z[t,y_t].
 //
 // Backward, in pieces of the vocabulary: the product again, with an epilogue that
 // turns each logit into d[t,v] = exp(z[t,v] - lse_t) - [v = y_t] and stores it in 16
-// bits, as [t][v] and as [v][t]; then dx += d W_piece (fp32) and dw_piece = d^T x.
+// bits; then dx += d W_piece (fp32) and dw_piece = d^T x, which read W, d and x as they
+// lie (line by line along the dimension that is summed over).
 //
 // Bound by the matrix cores: 2 T V H operations forward, 6 T V H backward (z is
 // computed again).  Logits, maxima, sums and the sums over tokens and vocabulary are
@@ -71,25 +72,24 @@ struct StatsEpilogue {
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq, int,
                                              uint8_t* lds) const {
     f32x2* all = reinterpret_cast<f32x2*>(lds);  // [wave along q][token of the tile]
-    __syncthreads();
     const int64_t v0 = row_q + t.q0();
     const bool whole = row_q + Tl::BQ <= vocab;
 #pragma unroll
-    for (int b = 0; b < Tl::PT; ++b) {
-      const int64_t token = row_p + t.p0() + 16 * b;
+    for (int b = 0; b < Tl::kColumns; ++b) {
+      const int64_t token = row_p + t.p0() + kLines * b;
       const int64_t y = token < tokens ? target[token] : -1;
       const int64_t rel64 = y - v0;
       const int rel = rel64 >= 0 && rel64 < Tl::BQ && y < vocab ? (int)rel64 : -1;
       float m = -INFINITY, hit = 0.0f;
       bool found = false;
 #pragma unroll
-      for (int a = 0; a < Tl::QT; ++a)
+      for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (!whole && v0 + 16 * a + i >= vocab) t.acc[a][b][i] = -INFINITY;
-          const float z = t.acc[a][b][i];
+          float z = t.quad(u, b)[i];
+          if (!whole && v0 + kLines * u + i >= vocab) z = -INFINITY;
           m = fmaxf(m, z);
-          if (rel == 16 * a + i) {
+          if (rel == kLines * u + i) {
             hit = z;
             found = true;
           }
@@ -98,13 +98,17 @@ struct StatsEpilogue {
       const float at = (m == -INFINITY ? 0.0f : m) * kLog2e;
       float s = 0.0f;
 #pragma unroll
-      for (int a = 0; a < Tl::QT; ++a)
+      for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += exp2_hw(fmaf(t.acc[a][b][i], kLog2e, -at));
+        for (int i = 0; i < 4; ++i) {
+          float z = t.quad(u, b)[i];
+          if (!whole && v0 + kLines * u + i >= vocab) z = -INFINITY;
+          s += exp2_hw(fmaf(z, kLog2e, -at));
+        }
       // the four lanes that hold this token's logits
       join(m, s, __shfl_xor(m, 16, kWave), __shfl_xor(s, 16, kWave));
       join(m, s, __shfl_xor(m, 32, kWave), __shfl_xor(s, 32, kWave));
-      if (t.lane < 16) all[t.wq * Tl::BP + t.p0() + 16 * b] = f32x2{m, s};
+      if (t.lane < kLines) all[t.wq * Tl::BP + t.p0() + kLines * b] = f32x2{m, s};
     }
     __syncthreads();
     for (int i = threadIdx.x; i < Tl::BP; i += Tl::kThreads) {
@@ -187,33 +191,35 @@ ce_reduce_kernel(const float* __restrict__ block_sum, const int* __restrict__ bl
 
 // ------------------------------------------------------------------ backward
 
-// Factors of a token.  The 16-bit d has to survive in fp16 too, whose smallest
-// normal number (6e-5) is far above a probability times a gradient of 1 / tokens:
-// there d is held times 2^15, and in [v][t] relative to the largest gradient.
+// Factors of a token with gradient g.  bf16: d is stored times g, and everything else is
+// 1.  fp16, whose smallest normal number (6e-5) is far above a probability times a
+// gradient of 1 / tokens: g = top m 2^e with top the largest |g| of all tokens and
+// 1/2 < |m| <= 1; d is stored times 2^15 m, x times 2^e (exactly, but for its smallest
+// numbers), and the rest goes into the fp32 sums.
 struct TokenFactors {
-  float* held;    // d -> [v][t]; 0: the token takes no part
-  float* dx;      // sum over v -> dx
-  float* dw;      // one element: sum over t -> dw
+  float* d;   // of d as it is stored; 0: the token takes no part
+  float* x;   // of x for dw
+  float* dx;  // of the sum over v
+  float* dw;  // one element: of the sum over t
 };
 constexpr float kF16Lift = 32768.0f;
 
 __global__ void __launch_bounds__(kReduceThreads)
 ce_factors_kernel(const float* __restrict__ grad, int per_token, int mean,
                   const float* __restrict__ count, const int64_t* __restrict__ target,
-                  int64_t tokens, int64_t padded, int64_t vocab, int64_t ignore, int f16,
-                  TokenFactors f) {
+                  int64_t tokens, int64_t vocab, int64_t ignore, int f16, TokenFactors f) {
   __shared__ float tops[kReduceThreads / kWave];
-  const float lift = f16 ? kF16Lift : 1.0f;
   float top = 0.0f;
-  for (int64_t i = threadIdx.x; i < padded; i += kReduceThreads) {
+  for (int64_t i = threadIdx.x; i < tokens; i += kReduceThreads) {
+    const int64_t y = target[i];
     float g = 0.0f;
-    if (i < tokens && target[i] != ignore) {
+    if (y != ignore) {
       g = grad[per_token ? i : 0];
       if (mean) g = g / *count;
-      if (target[i] < 0 || target[i] >= vocab) g = NAN;
+      if (y < 0 || y >= vocab) g = NAN;
     }
-    f.held[i] = g;
-    f.dx[i] = g / lift;
+    f.d[i] = g;
+    if (!f16) f.x[i] = f.dx[i] = g == 0.0f ? 0.0f : 1.0f;
     top = fmaxf(top, fabsf(g));
   }
   if (!f16) {
@@ -224,11 +230,20 @@ ce_factors_kernel(const float* __restrict__ grad, int per_token, int mean,
   if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
   __syncthreads();
   for (int w = 0; w < kReduceThreads / kWave; ++w) top = fmaxf(top, tops[w]);
-  if (threadIdx.x == 0) *f.dw = top / lift;
-  // each lane rescales what it wrote itself
-  for (int64_t i = threadIdx.x; i < padded; i += kReduceThreads) {
-    const float g = f.held[i];
-    if (g != 0.0f) f.held[i] = g / top * lift;
+  if (threadIdx.x == 0) *f.dw = top / kF16Lift;
+  // each lane goes over what it wrote itself
+  for (int64_t i = threadIdx.x; i < tokens; i += kReduceThreads) {
+    const float g = f.d[i];
+    int e = 0;
+    float m = g == 0.0f ? 0.0f : frexpf(g / top, &e);
+    if (fabsf(m) == 0.5f) {
+      m *= 2.0f;
+      e -= 1;
+    }
+    const float power = ldexpf(1.0f, e);
+    f.d[i] = m * kF16Lift;
+    f.x[i] = g == 0.0f ? 0.0f : power;
+    f.dx[i] = top * power / kF16Lift;
   }
 }
 
@@ -236,50 +251,44 @@ template <class T>
 struct ProbEpilogue {
   const int64_t* target;
   const float* lse;
-  const float* held;
-  int64_t tokens, vocab;  // of the piece: targets and columns count from its first row
-  int64_t first;          // first vocabulary row of the piece
-  uint16_t* d;            // [token][ld_d]
-  uint16_t* d_t;          // [vocabulary row of the piece][ld_t]
-  int64_t ld_d, ld_t;
-  float lift;
+  const float* factor;
+  int64_t tokens, rows;  // rows of the piece
+  int64_t first;         // its first vocabulary row
+  uint16_t* d;           // [token][ld]
+  int64_t ld;
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
-                                             uint8_t*) const {
+                                             uint8_t* lds) const {
     const int64_t v0 = row_q + t.q0();
+    const int left = rows - v0 < Tl::BQ ? (int)(rows - v0) : Tl::BQ;  // columns there are
+    float h[Tl::kColumns], at[Tl::kColumns];
+    int rel[Tl::kColumns];
 #pragma unroll
-    for (int b = 0; b < Tl::PT; ++b) {
-      const int64_t token = row_p + t.p0() + 16 * b;
+    for (int b = 0; b < Tl::kColumns; ++b) {
+      const int64_t token = row_p + t.p0() + kLines * b;
       const bool here = token < tokens;
-      const float h = here ? held[token] : 0.0f;
-      const bool used = h != 0.0f;
-      const float at = (here ? lse[token] : 0.0f) * kLog2e;
-      const int64_t rel64 = (here ? target[token] - first : -1) - v0;
-      const int rel = rel64 >= 0 && rel64 < Tl::BQ ? (int)rel64 : -1;
-#pragma unroll
-      for (int a = 0; a < Tl::QT; ++a) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float p = exp2_hw(fmaf(t.acc[a][b][i], kLog2e, -at));
-          if (rel == 16 * a + i) p -= 1.0f;
-          v[i] = used && v0 + 16 * a + i < vocab ? p : 0.0f;
-        }
-        const u32x2 w = {Store16<T>::pack(v[0] * lift, v[1] * lift),
-                         Store16<T>::pack(v[2] * lift, v[3] * lift)};
-        if (d) *reinterpret_cast<u32x2*>(d + token * ld_d + v0 + 16 * a) = w;
-        if (d_t) {
-          const u32x2 u = {Store16<T>::pack(v[0] * h, v[1] * h),
-                           Store16<T>::pack(v[2] * h, v[3] * h)};
-          uint16_t* o = d_t + (v0 + 16 * a) * ld_t + token;
-          o[0] = (uint16_t)u[0];
-          o[ld_t] = (uint16_t)(u[0] >> 16);
-          o[2 * ld_t] = (uint16_t)u[1];
-          o[3 * ld_t] = (uint16_t)(u[1] >> 16);
-        }
-      }
+      h[b] = here ? factor[token] : 0.0f;
+      at[b] = (here ? lse[token] : 0.0f) * kLog2e;
+      const int64_t r = (here ? target[token] - first : -1) - v0;
+      rel[b] = r >= 0 && r < Tl::BQ ? (int)r : -1;
     }
+    t.rows16(
+        lds,
+        [&](int u, int b) {
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int q = kLines * u + i;
+            float p = exp2_hw(fmaf(t.quad(u, b)[i], kLog2e, -at[b]));
+            if (rel[b] == q) p -= 1.0f;
+            v[i] = h[b] != 0.0f && q < left ? p * h[b] : 0.0f;
+          }
+          return u32x2{Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
+        },
+        [&](int p, int q, u32x4 v) {
+          if (row_p + p < tokens) *reinterpret_cast<u32x4*>(d + (row_p + p) * ld + row_q + q) = v;
+        });
   }
 };
 
@@ -291,22 +300,13 @@ struct SumEpilogue {
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int slice,
-                                             uint8_t*) const {
-    float* base = sum + (int64_t)slice * tokens * hidden;
-#pragma unroll
-    for (int b = 0; b < Tl::PT; ++b) {
-      const int64_t token = row_p + t.p0() + 16 * b;
-      if (token >= tokens) continue;
-#pragma unroll
-      for (int a = 0; a < Tl::QT; ++a) {
-        const int64_t h = row_q + t.q0() + 16 * a;
-        if (h >= hidden) continue;  // hidden is a multiple of 8: four at a time
-        f32x4* o = reinterpret_cast<f32x4*>(base + token * hidden + h);
-        f32x4 v = t.acc[a][b];
-        if (!first) v += *o;
-        *o = v;
-      }
-    }
+                                             uint8_t* lds) const {
+    float* base = sum + ((int64_t)slice * tokens + row_p) * hidden + row_q;
+    t.rows32(lds, [&](int p, int q, f32x4 v) {
+      if (row_p + p >= tokens || row_q + q >= hidden) return;  // hidden is a multiple of 8
+      f32x4* o = reinterpret_cast<f32x4*>(base + p * hidden + q);
+      *o = first ? v : *o + v;
+    });
   }
 };
 
@@ -318,97 +318,77 @@ struct WeightGradEpilogue {
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
-                                             uint8_t*) const {
+                                             uint8_t* lds) const {
     const float f = *factor;
-#pragma unroll
-    for (int b = 0; b < Tl::PT; ++b) {
-      const int64_t row = row_p + t.p0() + 16 * b;
-      if (row >= rows) continue;
-#pragma unroll
-      for (int a = 0; a < Tl::QT; ++a) {
-        const int64_t h = row_q + t.q0() + 16 * a;
-        if (h >= hidden) continue;
-        const f32x4 v = t.acc[a][b] * f;
-        const u32x2 w = {Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
-        *reinterpret_cast<u32x2*>(dw + row * hidden + h) = w;
-      }
-    }
+    t.rows16(
+        lds,
+        [&](int u, int b) {
+          const f32x4 v = t.quad(u, b) * f;
+          return u32x2{Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
+        },
+        [&](int p, int q, u32x4 v) {
+          if (row_p + p < rows && row_q + q < hidden)
+            *reinterpret_cast<u32x4*>(dw + (row_p + p) * hidden + row_q + q) = v;
+        });
   }
 };
 
 // Slices of the fp32 sums -> dx in 16 bits, four elements per lane.
 template <class T>
 __global__ void __launch_bounds__(256)
-ce_dx_kernel(const float* __restrict__ sum, int slices, const float* __restrict__ held,
-             const float* __restrict__ factor, int64_t tokens, int64_t hidden,
-             uint16_t* __restrict__ dx) {
+ce_dx_kernel(const float* __restrict__ sum, int slices, const float* __restrict__ factor,
+             int64_t tokens, int64_t hidden, uint16_t* __restrict__ dx) {
   const int64_t quads = tokens * hidden / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
-  const int64_t token = i * 4 / hidden;
+  const float f = factor[i * 4 / hidden];
   f32x4 v = reinterpret_cast<const f32x4*>(sum)[i];
   for (int s = 1; s < slices; ++s) v += reinterpret_cast<const f32x4*>(sum)[s * quads + i];
-  v = held[token] == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * factor[token];
+  v = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * f;
   reinterpret_cast<u32x2*>(dx)[i] =
       u32x2{Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
 }
 
-// out[c][r] = in[r][c] of 16-bit elements, 64 x 64 per workgroup; rows from `rows` up
-// to ld_out, and rows whose keep[] is 0, read as zero.
-constexpr int kTrTile = 64;
-__global__ void __launch_bounds__(256)
-transpose16_kernel(const uint16_t* __restrict__ in, int64_t ld_in, int64_t rows, int64_t cols,
-                   const float* __restrict__ keep, uint16_t* __restrict__ out, int64_t ld_out) {
-  __shared__ uint16_t tile[kTrTile][kTrTile + 2];
-  const int64_t r0 = (int64_t)blockIdx.x * kTrTile, c0 = (int64_t)blockIdx.y * kTrTile;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {  // eight consecutive columns of a row per lane
-    const int i = threadIdx.x + 256 * k, r = i / 8, c = i % 8 * 8;
-    u16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (r0 + r < rows && c0 + c < cols && (!keep || keep[r0 + r] != 0.0f))
-      v = *reinterpret_cast<const u16x8*>(in + (r0 + r) * ld_in + c0 + c);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) tile[r][c + j] = v[j];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int i = threadIdx.x + 256 * k, c = i / 8, r = i % 8 * 8;
-    if (c0 + c >= cols) continue;
-    u16x8 v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = tile[r + j][c];
-    *reinterpret_cast<u16x8*>(out + (c0 + c) * ld_out + r0 + r) = v;
+template <class T>
+__device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
+  if (std::is_same<T, Bf16>::value) {
+    a = bf16lo_to_f32(w);
+    b = bf16hi_to_f32(w);
+  } else {
+    a = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+    b = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
   }
 }
 
-int transpose16(const void* in, int64_t ld_in, int64_t rows, int64_t cols, const float* keep,
-                void* out, int64_t ld_out, hipStream_t s) {
-  hipLaunchKernelGGL(transpose16_kernel,
-                     dim3((unsigned)(ld_out / kTrTile), (unsigned)tiles_along(cols, kTrTile)),
-                     dim3(256), 0, s, static_cast<const uint16_t*>(in), ld_in, rows, cols, keep,
-                     static_cast<uint16_t*>(out), ld_out);
-  return launch_status();
+// x for dw: each token's row times its factor; rows that take no part become zeros,
+// whatever they hold.  Eight elements per lane.
+template <class T>
+__global__ void __launch_bounds__(256)
+ce_x_kernel(const uint16_t* __restrict__ x, int64_t ldx, const float* __restrict__ factor,
+            int64_t tokens, int64_t hidden, uint16_t* __restrict__ out) {
+  const int64_t per_row = hidden / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= tokens * per_row) return;
+  const int64_t token = i / per_row, c = i % per_row * 8;
+  const float f = factor[token];
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (f != 0.0f) {
+    w = *reinterpret_cast<const u32x4*>(x + token * ldx + c);
+    if (f != 1.0f)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpack<T>(w[k], a, b);
+        w[k] = Store16<T>::pack(a * f, b * f);
+      }
+  }
+  *reinterpret_cast<u32x4*>(out + token * hidden + c) = w;
 }
 
 // --------------------------------------------------------------- host side
 
-int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-
-// Carves a workspace; with a null base it only counts.
-struct Carver {
-  uint8_t* base;
-  size_t used = 0;
-  template <class P>
-  P* take(int64_t count) {
-    P* p = reinterpret_cast<P*>(base ? base + used : nullptr);
-    used += (size_t)up_to(count * (int64_t)sizeof(P), 256);
-    return p;
-  }
-};
-
 struct ForwardPlan {
-  bool large;
+  Cut cut;
   int tiles;
   int blocks;
   f32x2* part;
@@ -416,8 +396,8 @@ struct ForwardPlan {
   int* block_count;
   size_t bytes;
   ForwardPlan(int64_t tokens, int64_t vocab, void* ws) {
-    large = large_tiles_fill(vocab, tokens);
-    tiles = (int)tiles_along(vocab, large ? 256 : 128);
+    cut = cut_for(vocab, tokens > 0 ? tokens : 1, 0, false);
+    tiles = (int)tiles_along(vocab, cut.large ? 256 : 128);
     blocks = (int)tiles_along(tokens, kCombineTokens);
     Carver c{static_cast<uint8_t*>(ws)};
     part = c.take<f32x2>((int64_t)tiles * tokens);
@@ -428,44 +408,35 @@ struct ForwardPlan {
   }
 };
 
-// Elements of d that a piece of the vocabulary may hold: 64 Mi (128 MiB, twice).  A
-// larger piece saves passes over the fp32 sums of dx (one read and write per piece).
+// Elements of d that a piece of the vocabulary may hold: 64 Mi (128 MiB).  A larger
+// piece saves passes over the fp32 sums of dx (one read and write per piece).
 constexpr int64_t kPieceElems = (int64_t)64 << 20;
 
 struct BackwardPlan {
-  int64_t padded;       // tokens, rounded up to whole tiles
-  int64_t piece;        // vocabulary rows of a piece, whole tiles
-  int slices;           // of the dx product
-  float *held, *dx_factor, *dw_factor;
-  uint16_t *d, *d_t, *x_t, *w_t;
+  int64_t piece;  // vocabulary rows of a piece, whole tiles
+  Cut dx_cut;
+  TokenFactors f;
+  uint16_t *d, *x;
   float* sum;
   size_t bytes;
   BackwardPlan(int64_t tokens, int64_t hidden, int64_t vocab, bool want_dx, bool want_dw, void* ws) {
-    padded = up_to(tokens, 256);
     const int64_t whole = up_to(vocab, 256);
-    int64_t most = kPieceElems / padded / 256 * 256;
+    int64_t most = kPieceElems / tokens / 256 * 256;
     if (most < 256) most = 256;
-    const int64_t pieces = tiles_along(whole, (int)(most < whole ? most : whole));
-    piece = up_to(tiles_along(whole, (int)pieces), 256);
-    slices = slices_for(hidden, tokens, piece * 2);
+    if (most > whole) most = whole;
+    piece = up_to(tiles_along(whole, tiles_along(whole, most)), 256);
+    dx_cut = cut_for(hidden, tokens, steps_of(piece * 2), true);
     Carver c{static_cast<uint8_t*>(ws)};
-    held = c.take<float>(padded);
-    dx_factor = c.take<float>(padded);
-    dw_factor = c.take<float>(1);
-    d = want_dx ? c.take<uint16_t>(padded * piece) : nullptr;
-    w_t = want_dx ? c.take<uint16_t>(hidden * piece) : nullptr;
-    sum = want_dx ? c.take<float>(slices * tokens * hidden) : nullptr;
-    d_t = want_dw ? c.take<uint16_t>(padded * piece) : nullptr;
-    x_t = want_dw ? c.take<uint16_t>(hidden * padded) : nullptr;
+    f.d = c.take<float>(tokens);
+    f.x = c.take<float>(tokens);
+    f.dx = c.take<float>(tokens);
+    f.dw = c.take<float>(1);
+    d = c.take<uint16_t>(tokens * piece);
+    sum = want_dx ? c.take<float>(dx_cut.slices * tokens * hidden) : nullptr;
+    x = want_dw ? c.take<uint16_t>(tokens * hidden) : nullptr;
     bytes = c.used;
   }
 };
-
-template <class T, class E>
-int product(const Problem& pr, bool large, int slices, const E& e, hipStream_t s) {
-  return large ? launch_tiles<Large<T>, E>(pr, slices, e, s)
-               : launch_tiles<Small<T>, E>(pr, slices, e, s);
-}
 
 struct Head {
   const uint8_t *x, *w;
@@ -476,8 +447,8 @@ struct Head {
 
 Problem logits_problem(const Head& h, int64_t first, int64_t rows) {
   Problem pr{};
-  pr.q = Operand{h.w + first * h.ldw * 2, h.ldw * 2, rows};
-  pr.p = Operand{h.x, h.ldx * 2, h.tokens};
+  pr.q = Operand{h.w + first * h.ldw * 2, h.ldw * 2, rows, 0};
+  pr.p = Operand{h.x, h.ldx * 2, h.tokens, 0};
   pr.k_bytes = (int)(h.hidden * 2);
   return pr;
 }
@@ -488,7 +459,7 @@ int forward(const Head& h, int reduction, float* loss, float* lse, float* count,
   const ForwardPlan plan(h.tokens, h.vocab, ws);
   if (h.tokens > 0) {
     const StatsEpilogue e{h.target, h.tokens, h.vocab, plan.part, plan.z_target};
-    int rc = product<T>(logits_problem(h, 0, h.vocab), plan.large, 1, e, s);
+    int rc = launch_product<T, false, false>(logits_problem(h, 0, h.vocab), plan.cut, e, s);
     if (rc) return rc;
     hipLaunchKernelGGL(ce_combine_kernel, dim3((unsigned)plan.blocks), dim3(kCombineThreads), 0, s,
                        plan.part, plan.z_target, h.target, h.tokens, h.vocab, h.ignore, plan.tiles,
@@ -507,54 +478,48 @@ template <class T>
 int backward(const Head& h, int reduction, const float* lse, const float* count,
              const float* grad, uint16_t* dx, uint16_t* dw, void* ws, hipStream_t s) {
   const BackwardPlan plan(h.tokens, h.hidden, h.vocab, dx != nullptr, dw != nullptr, ws);
-  const bool f16 = std::is_same<T, F16>::value;
-  const TokenFactors f{plan.held, plan.dx_factor, plan.dw_factor};
+  const TokenFactors& f = plan.f;
   hipLaunchKernelGGL(ce_factors_kernel, dim3(1), dim3(kReduceThreads), 0, s, grad,
                      (int)(reduction == OA_LOSS_NONE), (int)(reduction == OA_LOSS_MEAN), count,
-                     h.target, h.tokens, plan.padded, h.vocab, h.ignore, (int)f16, f);
+                     h.target, h.tokens, h.vocab, h.ignore, (int)std::is_same<T, F16>::value, f);
   int rc = launch_status();
   if (rc) return rc;
   if (dw) {
-    rc = transpose16(h.x, h.ldx, h.tokens, h.hidden, plan.held, plan.x_t, plan.padded, s);
+    hipLaunchKernelGGL(ce_x_kernel<T>, dim3((unsigned)tiles_along(h.tokens * h.hidden / 8, 256)),
+                       dim3(256), 0, s, reinterpret_cast<const uint16_t*>(h.x), h.ldx, f.x,
+                       h.tokens, h.hidden, plan.x);
+    rc = launch_status();
     if (rc) return rc;
   }
   for (int64_t first = 0; first < h.vocab; first += plan.piece) {
     const int64_t rows = h.vocab - first < plan.piece ? h.vocab - first : plan.piece;
-    Problem pr = logits_problem(h, first, rows);
-    const bool large = large_tiles_fill(rows, h.tokens);
-    const ProbEpilogue<T> pe{h.target, lse,      plan.held,  h.tokens, rows,
-                             first,    plan.d,   plan.d_t,   plan.piece, plan.padded,
-                             f16 ? kF16Lift : 1.0f};
-    rc = product<T>(pr, large, 1, pe, s);
+    const ProbEpilogue<T> pe{h.target, lse, f.d, h.tokens, rows, first, plan.d, plan.piece};
+    rc = launch_product<T, false, false>(logits_problem(h, first, rows),
+                                         cut_for(rows, h.tokens, 0, false), pe, s);
     if (rc) return rc;
-    const int64_t tile = large ? 256 : 128;
     if (dx) {
-      rc = transpose16(h.w + first * h.ldw * 2, h.ldw, rows, h.hidden, nullptr, plan.w_t,
-                       plan.piece, s);
-      if (rc) return rc;
       Problem px{};
-      px.q = Operand{reinterpret_cast<uint8_t*>(plan.w_t), plan.piece * 2, h.hidden};
-      px.p = Operand{reinterpret_cast<uint8_t*>(plan.d), plan.piece * 2, h.tokens};
-      px.k_bytes = (int)(up_to(rows, tile) * 2);
+      px.q = Operand{h.w + first * h.ldw * 2, h.ldw * 2, h.hidden, rows};
+      px.p = Operand{reinterpret_cast<uint8_t*>(plan.d), plan.piece * 2, h.tokens, 0};
+      px.k_bytes = (int)(up_to(rows, 8) * 2);
       const SumEpilogue se{plan.sum, h.tokens, h.hidden, (int)(first == 0)};
-      rc = product<T>(px, plan.slices == 1 && large_tiles_fill(h.hidden, h.tokens), plan.slices,
-                      se, s);
+      rc = launch_product<T, true, false>(px, plan.dx_cut, se, s);
       if (rc) return rc;
     }
     if (dw) {
       Problem pw{};
-      pw.q = Operand{reinterpret_cast<uint8_t*>(plan.x_t), plan.padded * 2, h.hidden};
-      pw.p = Operand{reinterpret_cast<uint8_t*>(plan.d_t), plan.padded * 2, rows};
-      pw.k_bytes = (int)(up_to(h.tokens, tile) * 2);
-      const WeightGradEpilogue<T> we{dw + first * h.hidden, rows, h.hidden, plan.dw_factor};
-      rc = product<T>(pw, large_tiles_fill(h.hidden, rows), 1, we, s);
+      pw.q = Operand{reinterpret_cast<uint8_t*>(plan.x), h.hidden * 2, h.hidden, h.tokens};
+      pw.p = Operand{reinterpret_cast<uint8_t*>(plan.d), plan.piece * 2, rows, h.tokens};
+      pw.k_bytes = (int)(up_to(h.tokens, 8) * 2);
+      const WeightGradEpilogue<T> we{dw + first * h.hidden, rows, h.hidden, f.dw};
+      rc = launch_product<T, true, true>(pw, cut_for(h.hidden, rows, 0, false), we, s);
       if (rc) return rc;
     }
   }
   if (dx) {
     const int64_t quads = h.tokens * h.hidden / 4;
     hipLaunchKernelGGL(ce_dx_kernel<T>, dim3((unsigned)tiles_along(quads, 256)), dim3(256), 0, s,
-                       plan.sum, plan.slices, plan.held, plan.dx_factor, h.tokens, h.hidden, dx);
+                       plan.sum, plan.dx_cut.slices, f.dx, h.tokens, h.hidden, dx);
     rc = launch_status();
   }
   return rc;
@@ -585,7 +550,8 @@ extern "C" size_t oa_linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, i
   if (tokens < 0 || hidden <= 0 || vocab <= 0) return 0;
   // never 0: the workspace of an empty batch is a valid pointer too
   if (!backward) return ForwardPlan(tokens, vocab, nullptr).bytes + 256;
-  return BackwardPlan(tokens, hidden, vocab, want_dx != 0, want_dw != 0, nullptr).bytes + 256;
+  if (tokens == 0) return 0;
+  return BackwardPlan(tokens, hidden, vocab, want_dx != 0, want_dw != 0, nullptr).bytes;
 }
 
 extern "C" int oa_linear_ce_forward(const void* x, int64_t ldx, const void* w, int64_t ldw,

@@ -3,17 +3,35 @@
 //
 //     out[p][q] = sum_k P[p][k] * Q[q][k]          (both operands contiguous along k)
 //
-// A workgroup owns a BP x BQ tile of `out` and walks k in steps of 128 bytes per
-// row (64 bf16 / fp16 or 128 e4m3 elements).  Both operands' next step travels
-// from HBM to LDS with 16-byte direct loads (no registers in between) while the
-// current one is multiplied; LDS holds two steps.  A row of a step is eight
-// 16-byte chunks; chunk c of row r sits at position c ^ (r & 7), which spreads the
-// eight rows that a quarter-wave reads together over all banks.  A direct load
-// writes LDS in lane order, so the permutation is applied to the source address.
+// A workgroup of four waves owns a BP x BQ tile of `out`, each wave a quarter, and
+// walks k in steps of 128 bytes per row (64 bf16 / fp16 or 128 e4m3 elements).
+// Operands travel from HBM to LDS with 16-byte direct loads, no registers in between.
 //
-// A lane of a matrix instruction supplies chunks l/16 and l/16 + 4 of row l%16.
-// Which k elements those are does not matter as long as both operands agree, so
-// the three element types share every address computation.
+// What bounds it: with 256 x 256 the matrix cores need 2048 cycles a step, reading the
+// fragments takes 1024 of LDS time and filling LDS 512 (and 1024 of the L1's).  Eight
+// waves of 128 x 64 would read half as much again, which with the fills is all of LDS
+// time: 1060 TFLOP/s in bf16 at 4096 x 4096 x 8192 against 1220 for four waves with
+// the same loop.  One wave per SIMD has to overlap by itself: the products of one half
+// of a step (64 bytes of k) are interleaved by hand with the fragment reads of the
+// next half and with the loads of a later step, and the one barrier of a step sits
+// between the halves, where all of the step's fragments have been read.
+//
+// LDS is a ring of units, each the rows of one operand and one step that a wave needs
+// (four units to a step, ten or, with scales, nine in the ring): behind the step being
+// multiplied and the next one, two or one more units can be in flight while a step's
+// first half runs, and the rest follow into the units that the barrier frees.  The L1
+// delivers 64 bytes a cycle, half of what it could in a step: loads bunched into one half
+// would take all of its time.
+//
+// A row of a step is eight 16-byte chunks; chunk c of row r sits at position
+// c ^ (r / 2 % 8): the 16 lanes whose 16-byte reads LDS serves in one cycle hold rows of
+// both parities from eight different pairs, and touch each of the 64 banks once.  (With
+// c ^ (r % 8) half of the read cycles were bank conflicts: hidden, but they cost power,
+// which is what the clock follows here.)  A direct load writes LDS in lane order, so the
+// permutation is applied to the source address.  A lane of a matrix instruction supplies
+// chunk l/16 of a half of row l%16 (e4m3: chunks l/16 and l/16 + 4).  Which k elements
+// those are does not matter as long as both operands agree, so the element types share
+// every address.
 //
 // Q is the first operand of the matrix instruction: a lane then holds four
 // consecutive q of one p, which is the contiguous direction of `out`.
@@ -27,35 +45,60 @@
 namespace oa {
 namespace gemm {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStepBytes = 128;  // bytes of one row that one k step covers
-constexpr int kChunks = kStepBytes / 16;
+constexpr int kLines = 16;       // rows and columns of a matrix instruction
 
+// The instructions are written out because the compiler, short of registers, gives
+// their results other registers than their accumulators and moves 256 of them about.
+// Accumulators live in the accumulation registers, an instruction is 16 or more
+// cycles from the next on the same ones, and settle() stands before their first
+// other use.
+//
+// All types take the 16 x 16 forms (k of 32 or, e4m3, 128).  For the same product 32 x 32
+// moves more registers of accumulators, and the power limit sets the clock: products of
+// bf16 alone ran at 1800 MHz with the one and 1590 with the other.
 struct Bf16 {
   static constexpr bool kScaled = false;
+  static constexpr bool kQPacked = true;
+  typedef i32x4 Frag;  // of one row and half a step
   template <int, int>
-  static __device__ __forceinline__ f32x4 mma(const i32x4 (&q)[2], const i32x4 (&p)[2], f32x4 c,
-                                              int, int) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[0]),
-                                                __builtin_bit_cast(bf16x8, p[0]), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q[1]),
-                                                   __builtin_bit_cast(bf16x8, p[1]), c, 0, 0, 0);
+  static __device__ __forceinline__ void mul(f32x4& c, const Frag& q, const Frag& p, int, int) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(q), "v"(p));
+  }
+  template <int, int>
+  static __device__ __forceinline__ void mul_load(f32x4& c, const Frag& q, const Frag& p, int, int,
+                                                  uint32_t to, int offset, const i32x4& rsrc) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen lds"
+        : "+a"(c)
+        : "v"(q), "v"(p), "s"(to), "v"(offset), "s"(rsrc)
+        : "m0");
   }
 };
 
 struct F16 {
   static constexpr bool kScaled = false;
+  static constexpr bool kQPacked = true;
+  typedef i32x4 Frag;
   template <int, int>
-  static __device__ __forceinline__ f32x4 mma(const i32x4 (&q)[2], const i32x4 (&p)[2], f32x4 c,
-                                              int, int) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, q[0]),
-                                               __builtin_bit_cast(f16x8, p[0]), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, q[1]),
-                                                  __builtin_bit_cast(f16x8, p[1]), c, 0, 0, 0);
+  static __device__ __forceinline__ void mul(f32x4& c, const Frag& q, const Frag& p, int, int) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(q), "v"(p));
+  }
+  template <int, int>
+  static __device__ __forceinline__ void mul_load(f32x4& c, const Frag& q, const Frag& p, int, int,
+                                                  uint32_t to, int offset, const i32x4& rsrc) {
+    asm volatile(
+        "s_mov_b32 m0, %3\n\t"
+        "v_mfma_f32_16x16x32_f16 %0, %1, %2, %0\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen lds"
+        : "+a"(c)
+        : "v"(q), "v"(p), "s"(to), "v"(offset), "s"(rsrc)
+        : "m0");
   }
 };
 
@@ -65,35 +108,55 @@ struct F16 {
 // one (the rest is cut off), and those sums and the accumulator in fp32.  That is some
 // 2^-14 of a result, under the rounding of the codes (2^-4 each) and of a 16-bit result;
 // multiplying decoded values instead would keep 24 bits at half the rate.
+// Q_PACKED: Q's scales are per row, else per block of 128 rows.
+template <bool Q_PACKED>
 struct E4m3 {
   static constexpr bool kScaled = true;
+  static constexpr bool kQPacked = Q_PACKED;
+  typedef i32x8 Frag;  // of one row and a whole step
   template <int BYTE_Q, int BYTE_P>
-  static __device__ __forceinline__ f32x4 mma(const i32x4 (&q)[2], const i32x4 (&p)[2], f32x4 c,
-                                              int sq, int sp) {
-    const i32x8 a = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    const i32x8 b = __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, BYTE_Q, sq, BYTE_P, sp);
+  static __device__ __forceinline__ void mul(f32x4& c, const Frag& q, const Frag& p, int sq, int sp) {
+    asm volatile(
+        "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        "op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]"
+        : "+a"(c)
+        : "v"(q), "v"(p), "v"(sq), "v"(sp), "n"(BYTE_Q & 1), "n"(BYTE_P & 1), "n"(BYTE_Q >> 1),
+          "n"(BYTE_P >> 1));
+  }
+  template <int BYTE_Q, int BYTE_P>
+  static __device__ __forceinline__ void mul_load(f32x4& c, const Frag& q, const Frag& p, int sq,
+                                                  int sp, uint32_t to, int offset,
+                                                  const i32x4& rsrc) {
+    asm volatile(
+        "s_mov_b32 m0, %9\n\t"
+        "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        "op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0]\n\t"
+        "buffer_load_dwordx4 %10, %11, 0 offen lds"
+        : "+a"(c)
+        : "v"(q), "v"(p), "v"(sq), "v"(sp), "n"(BYTE_Q & 1), "n"(BYTE_P & 1), "n"(BYTE_Q >> 1),
+          "n"(BYTE_P >> 1), "s"(to), "v"(offset), "s"(rsrc)
+        : "m0");
   }
 };
 
-// An operand: rows of `ld` bytes (16-byte aligned), k_bytes of each taking part
-// (a multiple of 16).
+// An operand: rows of `ld` bytes (16-byte aligned), k_bytes of each taking part (a
+// multiple of 16); or, of 16-bit types, the other way round: `lines` lines of `ld` bytes,
+// one for each k, that hold one element of every row.
 struct Operand {
   const uint8_t* base;
   int64_t ld;
   int64_t rows;
+  int64_t lines;
 };
 
-// Where the scales of an e4m3 operand are.  `packed`: one byte per row and step, as
+// Where the scales of an e4m3 operand are.  Packed: one byte per row and step, as
 // [step][row group of 64][16] dwords, byte j of dword i = row 16 j + i of the group,
-// so that a lane's dword serves four matrix tiles; rows go up to a multiple of 256.
-// Otherwise one byte per 128 rows and step.
+// so that a lane's dword serves four matrix tiles; rows go up to a multiple of 256.  Else one byte per block of 128 rows and step.
 struct Scales {
   const uint8_t* base;
   int64_t step_stride;   // bytes from one step to the next
   int64_t block_stride;  // not packed: bytes from one block of 128 rows to the next
   int64_t blocks;        // not packed: number of those
-  bool packed;
 };
 
 // Byte of (row, step) in a packed array.
@@ -101,13 +164,22 @@ __host__ __device__ inline int64_t packed_scale_at(int64_t row, int64_t step, in
   return step * step_stride + row / 64 * 64 + row % 16 * 4 + row / 16 % 4;
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const Operand& o, int64_t row0,
-                                                            int tile_rows) {
+// Buffer descriptor: address, stride 0, bytes, raw 32-bit format; the same on every lane.
+__device__ __forceinline__ i32x4 descriptor(const uint8_t* base, int bytes) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  i32x4 r = {(int)(uint32_t)b, (int)(uint32_t)(b >> 32) & 0xFFFF, bytes, 0x00020000};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+  return r;
+}
+
+// Descriptor of a tile's rows from byte k of the first on: what is not in the range reads
+// as zero, among it every row past the operand's last.
+__device__ __forceinline__ i32x4 tile_rsrc(const Operand& o, int64_t row0, int tile_rows,
+                                           int64_t k) {
   int64_t rows = o.rows - row0;
   rows = rows < 0 ? 0 : (rows > tile_rows ? tile_rows : rows);
-  const uint8_t* base = o.base + (rows > 0 ? row0 * o.ld : 0);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)(rows * o.ld),
-                                           0x00020000);
+  return descriptor(o.base + (rows > 0 ? row0 * o.ld : 0) + k, (int)(rows * o.ld));
 }
 
 // The tile of workgroup b: consecutive workgroups go to the 8 XCDs in turn, and
@@ -129,160 +201,503 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_p, uint32_t t
   tq = in / wide;
 }
 
-template <class T, int BQ_, int BP_, int WQ, int WP>
+// KQ, KP: the operand lies line by line.  Its units are then lines of R elements, 64 of
+// them, and LDS hands the fragments out transposed (a lane gets four k of its row).  Tile t
+// (32 bytes) of a line sits at position t ^ f(line), which puts the lines that are read
+// together into different banks.
+template <class T, int B, bool KQ = false, bool KP = false>
 struct Tile {
-  static constexpr int BQ = BQ_, BP = BP_;
-  static constexpr int kWavesQ = WQ, kWavesP = WP, kWaves = WQ * WP, kThreads = kWave * kWaves;
-  static constexpr int QR = BQ / WQ, PR = BP / WP;  // rows of each operand that a wave owns
-  static constexpr int QT = QR / 16, PT = PR / 16;
-  static constexpr int kLoadsQ = BQ / 8 / kWaves, kLoadsP = BP / 8 / kWaves;
-  static constexpr int kBytesQ = BQ * kStepBytes, kBytesP = BP * kStepBytes;
-  static_assert(kLoadsQ * 8 * kWaves == BQ && kLoadsP * 8 * kWaves == BP, "tile / waves");
+  typedef T Type;
+  static_assert(!T::kScaled || (!KQ && !KP), "8-bit operands lie row by row");
+  static constexpr int BQ = B, BP = B;
+  static constexpr int kWavesQ = 2, kWaves = 4, kThreads = kWave * kWaves;
+  static constexpr int R = B / 2;        // rows of either operand that a wave multiplies: a unit
+  static constexpr int N = R / kLines;   // matrix tiles along either side of a wave's quarter
+  static constexpr int kUnitBytes = R * kStepBytes;
+  static constexpr int kLoads = R / 8 / kWaves;            // per wave and unit
+  static constexpr int kUnits = T::kScaled ? 9 : 10;
+  static constexpr int kEarly = kUnits - 8;                // units loaded in a step's first half
+  static constexpr int kScaleBytes = T::kScaled ? 512 : 0; // of a step: 64 dwords of q, 64 of p
+  static constexpr int kLdsBytes = kUnits * kUnitBytes + 3 * kScaleBytes;
+  static constexpr int kOut = 0x60000000;  // out of any descriptor's range
+  static_assert(R == 128 || R == 64, "scales come in groups of 128 rows");
 
-  f32x4 acc[QT][PT];
+  // A lane's results: kQuads groups of four consecutive q for each of kColumns p; quad u
+  // starts at q0() + 16 u, column b is p0() + 16 b.
+  static constexpr int kQuads = N, kColumns = N;
+  f32x4 acc[N][N];
   int lane, wave, wq, wp;
 
   __device__ __forceinline__ Tile() {
     lane = threadIdx.x & (kWave - 1);
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    wq = wave % WQ;
-    wp = wave / WQ;
+    wq = wave % 2;
+    wp = wave / 2;
+  }
+  __device__ __forceinline__ int q0() const { return wq * R + 4 * (lane / kLines); }
+  __device__ __forceinline__ int p0() const { return wp * R + lane % kLines; }
+  __device__ __forceinline__ const f32x4& quad(int u, int b) const { return acc[u][b]; }
+
+  // ---- halves of a step and their fragments.  16-bit: the halves are 64 bytes of k each,
+  // with fragments of their own.  e4m3, whose instruction takes all 128: the halves are
+  // the lower and the upper q tiles, with fragments of their own, and p's fragments serve
+  // both: in the second half each is read for the next step as soon as its products are
+  // issued, the last kLate of them at the beginning of that step.
+  static constexpr bool kHalvesOfK = !T::kScaled;
+  static constexpr int kPieces = kHalvesOfK ? 1 : 2;      // 16-byte chunks of a fragment
+  static constexpr int H = kHalvesOfK ? N : N / 2;        // q tiles of a half
+  static constexpr int kLate = N / 4;
+  static constexpr int kProducts = H * N;                 // of a half, p tiles outermost
+  struct Fragments {
+    typename T::Frag q[2][H], p[kHalvesOfK ? 2 : 1][N];
+    int sq[2], sp[2], next_sq[2], next_sp[2];  // scales, four tiles to a dword
+  };
+  int at[2];  // where this lane's chunks of the lower and the upper 64 bytes are in a unit
+  // ... and of an operand that lies line by line: where its piece of tile t of its line is
+  int at_line[N];
+  static constexpr int kLineBytes = R * 2;
+  static __device__ __forceinline__ int line_swizzle(int line) {
+    return R == 128 ? (line & 3) | (line >> 3 & 1) << 2 : (line >> 1 & 1) | (line >> 3 & 1) << 1;
   }
 
-  // First q / p of this lane's results relative to the tile: result i of acc[a][b]
-  // is (q0() + 16 a + i, p0() + 16 b).
-  __device__ __forceinline__ int q0() const { return wq * QR + 4 * (lane / 16); }
-  __device__ __forceinline__ int p0() const { return wp * PR + lane % 16; }
-
-  template <int N>
-  __device__ __forceinline__ void fetch(__amdgpu_buffer_rsrc_t rsrc, int ld, int step, int k_bytes,
-                                        uint8_t* lds) const {
-    const int c = (lane % 8) ^ (lane / 8);
-    const int k = step * kStepBytes + c * 16;
-    const int row = wave * N * 8 + lane / 8;
-    const int off = k < k_bytes ? row * ld + k : 0x7FFFFF00;
+  // Where this lane reads: its chunks of row 0 of either operand's unit, or its pieces of
+  // the tiles of its line.
+  struct From {
+    const uint8_t *q[KQ ? N : kPieces], *p[KP ? N : kPieces];
+  };
+  template <bool LINES, int COUNT>
+  __device__ __forceinline__ void from(const uint8_t* (&r)[COUNT], const uint8_t* lds, int half,
+                                       uint32_t unit) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc,
-          reinterpret_cast<__attribute__((address_space(3))) void*>(
-              reinterpret_cast<uintptr_t>(lds + (wave * N + i) * 8 * kStepBytes)),
-          16, k < k_bytes ? off + i * 8 * ld : off, 0, 0, 0);
+    for (int c = 0; c < COUNT; ++c)
+      r[c] = lds + (unit + (LINES ? at_line[c % N] : at[kHalvesOfK ? half : c % 2]));
   }
-
-  // Scales of this lane's rows, four 16-row tiles to a dword.
-  static constexpr int kScalesQ = (QT + 3) / 4, kScalesP = (PT + 3) / 4;
-
-  template <int A, int B>
-  __device__ __forceinline__ void multiply_row(const i32x4 (&fq)[2], const i32x4 (&fp)[PT][2],
-                                               const int (&sq)[kScalesQ],
-                                               const int (&sp)[kScalesP]) {
-    if constexpr (B < PT) {
-      acc[A][B] = T::template mma<A % 4, B % 4>(fq, fp[B], acc[A][B], sq[A / 4], sp[B / 4]);
-      multiply_row<A, B + 1>(fq, fp, sq, sp);
-    }
-  }
-
-  template <int A>
-  __device__ __forceinline__ void multiply_rows(const uint8_t* q, int o0, int o1,
-                                                const i32x4 (&fp)[PT][2],
-                                                const int (&sq)[kScalesQ],
-                                                const int (&sp)[kScalesP]) {
-    if constexpr (A < QT) {
-      i32x4 fq[2];
-      fq[0] = *reinterpret_cast<const i32x4*>(q + A * 16 * kStepBytes + o0);
-      fq[1] = *reinterpret_cast<const i32x4*>(q + A * 16 * kStepBytes + o1);
-      multiply_row<A, 0>(fq, fp, sq, sp);
-      multiply_rows<A + 1>(q, o0, o1, fp, sq, sp);
-    }
-  }
-
-  __device__ __forceinline__ void multiply(const uint8_t* lq, const uint8_t* lp,
-                                           const int (&sq)[kScalesQ], const int (&sp)[kScalesP]) {
-    const int r = lane % 16, g = lane / 16;
-    const uint8_t* q = lq + (wq * QR + r) * kStepBytes;
-    const uint8_t* p = lp + (wp * PR + r) * kStepBytes;
-    const int o0 = (g ^ (r & 7)) * 16, o1 = ((g + 4) ^ (r & 7)) * 16;
-    i32x4 fp[PT][2];
+  template <int I>
+  static __device__ __forceinline__ void put(typename T::Frag& f, const uint8_t* src, int row) {
+    const i32x4 v = *reinterpret_cast<const i32x4*>(src + row * kStepBytes);
 #pragma unroll
-    for (int b = 0; b < PT; ++b) {
-      fp[b][0] = *reinterpret_cast<const i32x4*>(p + b * 16 * kStepBytes + o0);
-      fp[b][1] = *reinterpret_cast<const i32x4*>(p + b * 16 * kStepBytes + o1);
-    }
-    multiply_rows<0>(q, o0, o1, fp, sq, sp);
+    for (int i = 0; i < 4; ++i) f[4 * I + i] = v[i];
   }
-
-  template <int N>
-  __device__ __forceinline__ void load_scales(const Scales& s, int64_t row0, int step,
-                                              int (&out)[N]) const {
-    if constexpr (T::kScaled) {
-      if (s.packed) {
-        const uint32_t* d = reinterpret_cast<const uint32_t*>(s.base + (int64_t)step * s.step_stride) +
-                            row0 / 64 * 16 + lane % 16;
-#pragma unroll
-        for (int j = 0; j < N; ++j) out[j] = (int)(d[16 * j] >> (8 * (row0 / 16 % 4)));
+  // Four k of this lane's row, from the pieces that the 16 lanes of its group point to.
+  template <int I>
+  static __device__ __forceinline__ void put_lines(typename T::Frag& f, const uint8_t* src) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(const_cast<uint8_t*>(src)));
+    const i32x2 w = __builtin_bit_cast(i32x2, v);
+    f[2 * I] = w[0];
+    f[2 * I + 1] = w[1];
+  }
+  // Fragments of half HALF, reads I ... of q's and of p's.
+  static constexpr int kReadsQ = KQ ? 2 * N : H * kPieces, kReadsP = KP ? 2 * N : N * kPieces;
+  template <int HALF, int I, int COUNT>
+  __device__ __forceinline__ void read_q(const From& r, Fragments& f) const {
+    if constexpr (COUNT > 0) {
+      if constexpr (KQ) {
+        put_lines<I % 2>(f.q[HALF][I / 2], r.q[I / 2] + (32 * HALF + 4 * (I % 2)) * kLineBytes);
       } else {
-        int64_t block = row0 / 128;  // a tile may hang over the last block
-        if (block >= s.blocks) block = s.blocks - 1;
-        const int v = s.base[block * s.block_stride + step * s.step_stride] * 0x01010101;
+        constexpr int t = I / kPieces, c = I % kPieces;
+        put<c>(f.q[HALF][t], r.q[c], (t + (kHalvesOfK ? 0 : HALF * H)) * kLines);
+      }
+      read_q<HALF, I + 1, COUNT - 1>(r, f);
+    }
+  }
+  template <int HALF, int I, int COUNT>
+  __device__ __forceinline__ void read_p(const From& r, Fragments& f) const {
+    if constexpr (COUNT > 0) {
+      if constexpr (KP) {
+        put_lines<I % 2>(f.p[HALF][I / 2], r.p[I / 2] + (32 * HALF + 4 * (I % 2)) * kLineBytes);
+      } else {
+        constexpr int t = I / kPieces, c = I % kPieces;
+        put<c>(f.p[kHalvesOfK ? HALF : 0][t], r.p[c], t * kLines);
+      }
+      read_p<HALF, I + 1, COUNT - 1>(r, f);
+    }
+  }
+  // The reads that go before product G of half HALF: the fragments of the next half.
+  static constexpr int spread(int g, int count, int first, int last) {  // how many before g
+    return g <= first ? 0 : g >= last ? count : (g - first) * count / (last - first);
+  }
+  static constexpr int kQuiet = kProducts < 16 ? 1 : kProducts / 8;  // at the end, no reads
+  template <int HALF, int G>
+  __device__ __forceinline__ void reads(const From& r, Fragments& f) const {
+    constexpr int next = HALF ^ 1, last = kProducts - kQuiet, nq = kReadsQ, np = kReadsP;
+    if constexpr (kHalvesOfK) {
+      constexpr int p0 = spread(G, np, 0, last / 2), p1 = spread(G + 1, np, 0, last / 2);
+      read_p<next, p0, p1 - p0>(r, f);
+      constexpr int q0 = spread(G, nq, last / 2, last), q1 = spread(G + 1, nq, last / 2, last);
+      read_q<next, q0, q1 - q0>(r, f);
+    } else if constexpr (HALF == 0) {
+      constexpr int late = 2 * kLate;
+      if constexpr (G < late) read_p<0, 2 * (N - kLate) + G, 1>(r, f);
+      constexpr int q0 = spread(G, nq, late, last), q1 = spread(G + 1, nq, late, last);
+      read_q<1, q0, q1 - q0>(r, f);
+    } else {
+      constexpr int t = G / H - 1, c = G % H;  // p tile t has no products left
+      if constexpr (t >= 0 && t < N - kLate && c < 2) read_p<0, 2 * t + c, 1>(r, f);
+      constexpr int q0 = spread(G, nq, 0, last), q1 = spread(G + 1, nq, 0, last);
+      read_q<0, q0, q1 - q0>(r, f);
+    }
+  }
+
+  // Scales of a step, from LDS.
+  __device__ __forceinline__ void read_scales(const uint8_t* s, int (&sq)[2], int (&sp)[2]) const {
+    if constexpr (T::kScaled) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) out[j] = v;
+      for (int g = 0; g < R / 64; ++g) {
+        const int i = lane % kLines * 4 + g * 64;
+        sq[g] = *reinterpret_cast<const int*>(s + wq * R + i);
+        sp[g] = *reinterpret_cast<const int*>(s + 256 + wp * R + i);
+      }
+    }
+  }
+
+  // ---- loads into LDS.  Written out because the compiler, seeing LDS written by a load
+  // in flight, would wait for it before every read of LDS that it cannot tell apart; the
+  // waits are in step().  Nothing is loaded into registers.
+  struct Walk {
+    i32x4 rsrc[2];  // q, p: a tile's rows, from the k of the step that is loaded next
+    int step_bytes[2];
+    int k_end, lines, last;
+    Scales sq, sp;
+    int64_t scale_row;  // of this wave: q's tile (even waves) or p's
+    // this lane's offsets of the loads of q's two units and of p's, the same in every step
+    // that is wholly there
+    int offset[2][2 * kLoads];
+  };
+  static __device__ __forceinline__ void load16(i32x4 rsrc, int offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to), "v"(offset), "s"(rsrc)
+                 : "m0");
+  }
+  // This lane's chunk in a row of load i of a unit: rows of odd loads hold their chunks
+  // four positions away from those of even ones.
+  __device__ __forceinline__ int chunk_of(int i) const {
+    return (lane % 8) ^ (lane / 16 + 4 * (i % 2));
+  }
+  // Load I of the four units of a step: q's two, then p's two.
+  template <int I>
+  static constexpr int operand_of() {
+    return I / (2 * kLoads);
+  }
+  // ... its place in a unit in LDS, and its offset in `step`: FULL steps are wholly there,
+  // of others chunks from k_end on read as zero.
+  template <int I>
+  __device__ __forceinline__ uint32_t place(uint32_t unit) const {
+    return unit + (wave * kLoads + I % kLoads) * 8 * kStepBytes;
+  }
+  template <int I, bool FULL>
+  __device__ __forceinline__ int offset_of(const Walk& w, int step) const {
+    constexpr int o = operand_of<I>(), i = I % kLoads;
+    const int offset = w.offset[o][I % (2 * kLoads)];
+    if (FULL) return offset;
+    if (o == 0 ? KQ : KP) return step * 64 + line_of(i) < w.lines ? offset : kOut;
+    return step * kStepBytes + chunk_of(i) * 16 < w.k_end ? offset : kOut;
+  }
+  // Load i of a unit that lies line by line: this lane's line.
+  __device__ __forceinline__ int line_of(int i) const {
+    constexpr int lanes = kLineBytes / 16;
+    return (wave * kLoads + i) * (kWave / lanes) + lane / lanes;
+  }
+  template <bool LINES>
+  __device__ __forceinline__ void start(Walk& w, int o, const Operand& op, int64_t row0, int step0) {
+    if constexpr (LINES) {
+      w.rsrc[o] = descriptor(op.base + (int64_t)step0 * 64 * op.ld + row0 * 2, 64 * (int)op.ld);
+      w.step_bytes[o] = 64 * (int)op.ld;
+#pragma unroll
+      for (int i = 0; i < 2 * kLoads; ++i) {
+        const int line = line_of(i % kLoads);
+        const int c = lane % (kLineBytes / 16) ^ 2 * line_swizzle(line);
+        const int row = i / kLoads * R + c * 8;
+        w.offset[o][i] = row0 + row < op.rows ? line * (int)op.ld + row * 2 : kOut;
       }
     } else {
+      w.rsrc[o] = tile_rsrc(op, row0, B, (int64_t)step0 * kStepBytes);
+      w.step_bytes[o] = kStepBytes;
 #pragma unroll
-      for (int j = 0; j < N; ++j) out[j] = 0;
+      for (int i = 0; i < 2 * kLoads; ++i) {
+        const int row = i / kLoads * R + (wave * kLoads + i % kLoads) * 8 + lane / 8;
+        w.offset[o][i] = row * (int)op.ld + chunk_of(i % kLoads) * 16;
+      }
+    }
+  }
+  template <int I>
+  __device__ __forceinline__ void load_all(const Walk& w, int step, uint32_t first) const {
+    if constexpr (I < 4 * kLoads) {
+      load16(w.rsrc[operand_of<I>()], offset_of<I, false>(w, step),
+             place<I>(first + I / kLoads * kUnitBytes));
+      load_all<I + 1>(w, step, first);
+    }
+  }
+  static __device__ __forceinline__ void advance(Walk& w) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      const uint64_t b =
+          ((uint64_t)(uint32_t)w.rsrc[o][1] << 32 | (uint32_t)w.rsrc[o][0]) +
+          (uint32_t)w.step_bytes[o];
+      w.rsrc[o][0] = (int)(uint32_t)b;
+      w.rsrc[o][1] = (int)(uint32_t)(b >> 32);
+    }
+  }
+  // Even waves bring q's scales of a step, odd ones p's (two waves the same bytes to the
+  // same place).
+  __device__ __forceinline__ void load_scales(const Walk& w, int step, uint32_t to) const {
+    if constexpr (T::kScaled) {
+      const int64_t s = step < w.last ? step : w.last;
+      const bool q = wave % 2 == 0;
+      const Scales& sc = q ? w.sq : w.sp;
+      if (q && !T::kQPacked) {
+        // one byte per block of 128 rows, as a dword to each of 32 lanes
+        int64_t block = w.scale_row / 128 + (R == 128 ? lane / 32 : 0);
+        if (block >= sc.blocks) block = sc.blocks - 1;  // a tile may hang over the last
+        const i32x4 rsrc = descriptor(sc.base + s * sc.step_stride,
+                                      (int)((sc.blocks - 1) * sc.block_stride + 1));
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, 0 offen lds"
+                     :
+                     : "s"(to), "v"((int)(block * sc.block_stride)), "s"(rsrc)
+                     : "m0");
+      } else {
+        const i32x4 rsrc = descriptor(sc.base + s * sc.step_stride + w.scale_row, 2 * R);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                     :
+                     : "s"(to + (q ? 0 : 256)), "v"(lane * 4), "s"(rsrc)
+                     : "m0");
+      }
     }
   }
 
-  // The products of steps [step0, step1) of the tile at (row_q, row_p).
+  // ---- the ring: units 0..3 of a step (q of the waves 0 and 1, p of the waves 0 and 1)
+  // start at its position, those of the next step follow, then those that are free.
+  static constexpr uint32_t kRing = kUnits * kUnitBytes;
+  static __device__ __forceinline__ uint32_t wrap(uint32_t v) { return v >= kRing ? v - kRing : v; }
+  struct State {
+    const uint8_t* lds;
+    uint32_t base;       // of it, as an LDS address
+    uint32_t position;   // of step s
+    uint32_t scales[3];  // of s, s + 1 and, free, s + 2
+    uint32_t fill;       // unit that the loads at hand go to, as an LDS address
+    From next;           // where the next half's fragments are
+    int ahead;           // step that is being loaded
+  };
+
+  // Half HALF of a step: its products and between them, evenly spread, the reads of the
+  // next half and this half's share of the loads of step s + 2.  A product occupies the
+  // matrix core for 16 cycles (e4m3: 32); two or three other instructions fit between it
+  // and the next, so the scalar work of a step is spread too.
+  static constexpr int kTurn = kProducts < 16 ? kProducts - 1 : kProducts - 3;
+  template <int HALF, int G, bool FULL>
+  __device__ __forceinline__ void half(Walk& w, State& st, Fragments& f) {
+    if constexpr (G < kProducts) {
+      reads<HALF, G>(st.next, f);
+      constexpr int from = HALF == 0 ? 0 : kEarly * kLoads;
+      constexpr int loads = (HALF == 0 ? kEarly : 4 - kEarly) * kLoads;
+      constexpr int l0 = G * loads / kProducts, l1 = (G + 1) * loads / kProducts;
+      constexpr int a = G % H, b = G / H, qa = a + (kHalvesOfK ? 0 : HALF * H);
+      constexpr int slot = kHalvesOfK ? HALF : 0, byte_q = T::kQPacked ? qa % 4 : 0;
+      const int sq = f.sq[qa / 4], sp = f.sp[b / 4];
+      if constexpr (l1 > l0) {
+        constexpr int I = from + l0;
+        static_assert(l1 - l0 <= 2, "a product takes one load along, one may go before it");
+        unit_of<I>(st);
+        if constexpr (l1 - l0 == 2) {
+          load16(w.rsrc[operand_of<I>()], offset_of<I, FULL>(w, st.ahead), place<I>(st.fill));
+          unit_of<I + 1>(st);
+        }
+        constexpr int L = from + l1 - 1;
+        T::template mul_load<byte_q, b % 4>(acc[qa][b], f.q[HALF][a], f.p[slot][b], sq, sp,
+                                            place<L>(st.fill), offset_of<L, FULL>(w, st.ahead),
+                                            w.rsrc[operand_of<L>()]);
+      } else {
+        T::template mul<byte_q, b % 4>(acc[qa][b], f.q[HALF][a], f.p[slot][b], sq, sp);
+      }
+      // behind the last reads: where the half after the next one reads
+      if constexpr (G == kTurn) {
+        if constexpr (HALF == 0) {
+          st.next = from_units(st, 0, wrap(st.position + 4 * kUnitBytes));
+        } else {
+          st.position = wrap(st.position + 4 * kUnitBytes);
+          st.next = from_units(st, 1, st.position);
+        }
+      }
+      if constexpr (G == kProducts - 1 && HALF == 1) {  // behind the last load
+        advance(w);
+        ++st.ahead;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      half<HALF, G + 1, FULL>(w, st, f);
+    }
+  }
+  __device__ __forceinline__ From from_units(const State& st, int half, uint32_t position) const {
+    From r;
+    from<KQ>(r.q, st.lds, half, wrap(position + wq * kUnitBytes));
+    from<KP>(r.p, st.lds, half, wrap(position + (2 + wp) * kUnitBytes));
+    return r;
+  }
+  // The first load of a unit finds out where it is.
+  template <int I>
+  __device__ __forceinline__ void unit_of(State& st) const {
+    if constexpr (I % kLoads == 0)
+      st.fill = st.base + wrap(st.position + (8 + I / kLoads) % kUnits * kUnitBytes);
+  }
+
+  // Step s: on entry the fragments of its first half are there.
+  template <bool FULL>
+  __device__ __forceinline__ void step(Walk& w, State& st, Fragments& f) {
+    load_scales(w, st.ahead, st.base + st.scales[2]);
+    half<0, 0, FULL>(w, st, f);
+    // all but this half's loads have landed, so step s + 1 is there; and this step's
+    // fragments are all read
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kEarly * kLoads + (T::kScaled ? 1 : 0))
+                 : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (T::kScaled) {
+      read_scales(st.lds + st.scales[1], f.next_sq, f.next_sp);
+      const uint32_t first = st.scales[0];
+      st.scales[0] = st.scales[1];
+      st.scales[1] = st.scales[2];
+      st.scales[2] = first;
+    }
+    half<1, 0, FULL>(w, st, f);
+    if constexpr (T::kScaled) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        f.sq[g] = f.next_sq[g];
+        f.sp[g] = f.next_sp[g];
+      }
+      // two wait states between a register's write by a vector instruction and its use by
+      // a matrix instruction, which the compiler cannot see in the text of the latter
+      asm volatile("s_nop 1" : "+v"(f.sq[0]), "+v"(f.sq[1]), "+v"(f.sp[0]), "+v"(f.sp[1]));
+    }
+    // The last reads are kQuiet products back.  Said here, so that the compiler does not
+    // wait at the head of the loop, behind the next step's first reads.
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  }
+
+  // ---- results through LDS, so that they leave in whole rows.  Stored straight from
+  // the accumulators a wave's store touches 32 rows with 16 bytes each: that took 32 us of
+  // a 264 us product of 4096 x 4096 x 8192 in bf16 and 64 of 280 at 4096 x 14336 x 4096
+  // in e4m3.
+
+  // 16-bit results: value(u, b) gives quad u of column b packed into two dwords, and
+  // sink(p, q, v) takes eight consecutive q of one p.
+  static constexpr int kRow16 = BQ * 2 + 16;  // bytes; the odd 16 spread the rows over banks
+  template <class V, class S>
+  __device__ __forceinline__ void rows16(uint8_t* lds, const V& value, const S& sink) const {
+#pragma unroll
+    for (int b = 0; b < kColumns; ++b)
+#pragma unroll
+      for (int u = 0; u < kQuads; ++u)
+        *reinterpret_cast<u32x2*>(lds + (p0() + kLines * b) * kRow16 + (q0() + kLines * u) * 2) =
+            value(u, b);
+    __syncthreads();
+    constexpr int lanes = BQ / 8, rows = kThreads / lanes;
+    const int q = threadIdx.x % lanes * 8;
+#pragma unroll 4
+    for (int p = threadIdx.x / lanes; p < BP; p += rows)
+      sink(p, q, *reinterpret_cast<const u32x4*>(lds + p * kRow16 + q * 2));
+  }
+
+  // fp32 results, the two halves of the rows one after the other: sink(p, q, v) takes
+  // four consecutive q of one p.
+  static constexpr int kRow32 = BQ * 4 + 16;
+  template <class S>
+  __device__ __forceinline__ void rows32(uint8_t* lds, const S& sink) const {
+    constexpr int lanes = BQ / 4, rows = kThreads / lanes;
+    const int q = threadIdx.x % lanes * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h) __syncthreads();
+      if (wp == h)
+#pragma unroll
+        for (int b = 0; b < kColumns; ++b)
+#pragma unroll
+          for (int u = 0; u < kQuads; ++u)
+            *reinterpret_cast<f32x4*>(lds + (lane % kLines + kLines * b) * kRow32 +
+                                      (q0() + kLines * u) * 4) = quad(u, b);
+      __syncthreads();
+#pragma unroll 4
+      for (int p = threadIdx.x / lanes; p < R; p += rows)
+        sink(h * R + p, q, *reinterpret_cast<const f32x4*>(lds + p * kRow32 + q * 4));
+    }
+  }
+  static_assert(BP * (BQ * 2 + 16) <= kLdsBytes && R * (BQ * 4 + 16) <= kLdsBytes, "epilogue");
+
+  // The matrix cores are done with the accumulators; and what follows stays behind this
+  // point, on every lane.
+  __device__ __forceinline__ void settle() {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int a = 0; a < N; ++a)
+#pragma unroll
+      for (int b = 0; b < N; ++b) asm volatile("" : "+a"(acc[a][b]));
+  }
+
+  // The products of steps [step0, step1) of the tile at (row_q, row_p); `lds` has
+  // kLdsBytes.  Ends with a barrier: LDS is free.
   __device__ __forceinline__ void run(const Operand& oq, const Operand& op, int64_t row_q,
                                       int64_t row_p, int k_bytes, int step0, int step1,
-                                      const Scales& scq, const Scales& scp, uint8_t* lq0,
-                                      uint8_t* lq1, uint8_t* lp0, uint8_t* lp1) {
+                                      const Scales& scq, const Scales& scp, uint8_t* lds) {
 #pragma unroll
-    for (int a = 0; a < QT; ++a)
+    for (int a = 0; a < N; ++a)
 #pragma unroll
-      for (int b = 0; b < PT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const auto rq = tile_rsrc(oq, row_q, BQ), rp = tile_rsrc(op, row_p, BP);
-    const int ldq = (int)oq.ld, ldp = (int)op.ld;
-    const int64_t mine_q = row_q + wq * QR, mine_p = row_p + wp * PR;
-    int sq[kScalesQ], sp[kScalesP], nsq[kScalesQ], nsp[kScalesP];
-    const int begin = step0 < step1 ? step0 : 0;  // an empty slice: any scale that is there
-    load_scales(scq, mine_q, begin, sq);
-    load_scales(scp, mine_p, begin, sp);
-    // steps from step1 on read as zero
-    const int k_end = k_bytes < step1 * kStepBytes ? k_bytes : step1 * kStepBytes;
-    fetch<kLoadsQ>(rq, ldq, step0, k_end, lq0);
-    fetch<kLoadsP>(rp, ldp, step0, k_end, lp0);
-    int s = step0;
-    for (; s + 1 < step1; s += 2) {
-      wait();
-      load_scales(scq, mine_q, s + 1, nsq);
-      load_scales(scp, mine_p, s + 1, nsp);
-      fetch<kLoadsQ>(rq, ldq, s + 1, k_end, lq1);
-      fetch<kLoadsP>(rp, ldp, s + 1, k_end, lp1);
-      multiply(lq0, lp0, sq, sp);
-      wait();
-      const int next = s + 2 < step1 ? s + 2 : s + 1;  // scales past the end are not there
-      load_scales(scq, mine_q, next, sq);
-      load_scales(scp, mine_p, next, sp);
-      fetch<kLoadsQ>(rq, ldq, s + 2, k_end, lq0);
-      fetch<kLoadsP>(rp, ldp, s + 2, k_end, lp0);
-      multiply(lq1, lp1, nsq, nsp);
-    }
-    wait();
-    if (s < step1) multiply(lq0, lp0, sq, sp);
-    // The results exist here, on every lane: a matrix instruction that moved into a
-    // branch of the epilogue would lose the operands of the lanes that do not take it.
+      for (int b = 0; b < N; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (step0 >= step1) return;
+    Walk w;
+    start<KQ>(w, 0, oq, row_q, step0);
+    start<KP>(w, 1, op, row_p, step0);
+    w.k_end = k_bytes < step1 * kStepBytes ? k_bytes : step1 * kStepBytes;
+    int full = w.k_end / kStepBytes;  // steps that are wholly there
+    w.lines = step1 * 64;
+    if (KQ && oq.lines < w.lines) w.lines = (int)oq.lines;
+    if (KP && op.lines < w.lines) w.lines = (int)op.lines;
+    if ((KQ || KP) && w.lines / 64 < full) full = w.lines / 64;
+    w.last = step1 - 1;
+    w.sq = scq;
+    w.sp = scp;
+    w.scale_row = wave % 2 == 0 ? row_q : row_p;
 #pragma unroll
-    for (int a = 0; a < QT; ++a)
+    for (int i = 0; i < 2; ++i)
+      at[i] = lane % kLines * kStepBytes + ((lane / kLines + 4 * i) ^ (lane / 2 % 8)) * 16;
+    const int line = lane / kLines * 8 + lane % kLines / 4;
 #pragma unroll
-      for (int b = 0; b < PT; ++b) asm volatile("" : "+v"(acc[a][b]));
-  }
+    for (int t = 0; t < N; ++t)
+      at_line[t] = line * kLineBytes + (t ^ line_swizzle(line)) * 32 + lane % 4 * 8;
 
-  // This wave's direct loads have landed in LDS, and every wave of the workgroup has
-  // come this far: its loads have landed too, and it is done reading the other buffers.
-  static __device__ __forceinline__ void wait() {
+    const uint32_t base = __builtin_amdgcn_readfirstlane(
+        (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    State st;
+    st.lds = lds;
+    st.base = base;
+    st.position = 0;
+    st.fill = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) st.scales[i] = kRing + i * kScaleBytes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_scales(w, step0 + i, base + st.scales[i]);
+      load_all<0>(w, step0 + i, base + 4 * i * kUnitBytes);
+      advance(w);
+    }
+    st.ahead = step0 + 2;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * kLoads + (T::kScaled ? 1 : 0)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Fragments f;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) f.sq[g] = f.sp[g] = f.next_sq[g] = f.next_sp[g] = 0;
+    read_scales(lds + st.scales[0], f.sq, f.sp);
+    st.next = from_units(st, 0, 0);
+    read_q<0, 0, kReadsQ>(st.next, f);
+    read_p<0, 0, kHalvesOfK ? kReadsP : 2 * (N - kLate)>(st.next, f);
+    st.next = from_units(st, 1, 0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    while (st.ahead < full) step<true>(w, st, f);
+    while (st.ahead < step1 + 2) step<false>(w, st, f);
+    settle();
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -303,8 +718,7 @@ inline int steps_of(int64_t k_bytes) { return (int)((k_bytes + kStepBytes - 1) /
 
 template <class T, class E>
 __global__ void __launch_bounds__(T::kThreads) product_kernel(const Problem pr, const E epilogue) {
-  __shared__ __align__(16) uint8_t lq0[T::kBytesQ], lq1[T::kBytesQ];
-  __shared__ __align__(16) uint8_t lp0[T::kBytesP], lp1[T::kBytesP];
+  __shared__ __align__(16) uint8_t lds[T::kLdsBytes];
   T t;
   uint32_t tp, tq;
   const uint32_t tiles = pr.tiles_p * pr.tiles_q;
@@ -314,35 +728,50 @@ __global__ void __launch_bounds__(T::kThreads) product_kernel(const Problem pr, 
   const int steps = (pr.k_bytes + kStepBytes - 1) / kStepBytes;
   const int step0 = (int)slice * pr.steps_per_slice;
   const int step1 = step0 + pr.steps_per_slice < steps ? step0 + pr.steps_per_slice : steps;
-  t.run(pr.q, pr.p, row_q, row_p, pr.k_bytes, step0, step1, pr.sq, pr.sp, lq0, lq1, lp0, lp1);
-  epilogue(t, row_q, row_p, (int)tq, (int)slice, lq0);
+  t.run(pr.q, pr.p, row_q, row_p, pr.k_bytes, step0, step1, pr.sq, pr.sp, lds);
+  epilogue(t, row_q, row_p, (int)tq, (int)slice, lds);
 }
 
-// Tile sizes.  256 x 256 with 8 waves reads each byte of LDS for 2 (q) or 4 (p)
-// waves and is the fastest where it fills the chip; with fewer tiles than three
-// quarters of the 256 CUs the 128 x 128 tile, two workgroups to a CU, leaves fewer
-// of them idle.  Measured in bf16: 4096 x 14336 x 4096 takes 471 us with the large
-// tile and 539 us with the small one; 1000 x 1020 x 520 takes 17.7 against 8.4 us.
-template <class T>
-using Large = Tile<T, 256, 256, 2, 4>;
-template <class T>
-using Small = Tile<T, 128, 128, 2, 2>;
-constexpr int64_t kFillTiles = 192;
+// Tile sizes: 256 x 256, one workgroup to a CU, and 128 x 128, two to a CU.  A step of
+// the two small ones takes a CU about as long as their half of the large one's, but reads
+// twice the bytes from L2 and LDS for it, and power is what the clock follows: 222 against
+// 267 us in bf16 at 4096 x 4096 x 8192.
+template <class T, bool KQ = false, bool KP = false>
+using Large = Tile<T, 256, KQ, KP>;
+template <class T, bool KQ = false, bool KP = false>
+using Small = Tile<T, 128, KQ, KP>;
 
-inline int64_t tiles_along(int64_t rows, int tile) { return (rows + tile - 1) / tile; }
+inline int64_t tiles_along(int64_t rows, int64_t tile) { return (rows + tile - 1) / tile; }
 
-inline bool large_tiles_fill(int64_t rows_q, int64_t rows_p) {
-  return tiles_along(rows_q, 256) * tiles_along(rows_p, 256) >= kFillTiles;
-}
+// How a product is cut: into which tiles, and each tile along k into how many slices.
+struct Cut {
+  bool large;
+  int slices;
+};
 
-// Workgroups that share a tile along k: enough that the chip is filled, no slice
-// shorter than 8 steps (a slice pays one pass over its partial results).
-inline int slices_for(int64_t rows_q, int64_t rows_p, int64_t k_bytes) {
-  const int64_t tiles = tiles_along(rows_q, 128) * tiles_along(rows_p, 128);
-  int64_t s = 2 * kFillTiles / tiles;
-  const int64_t most = steps_of(k_bytes) / 8;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s);
+// Whichever of the two tiles leaves less of the chip idle, the large one counted 1.2-fold:
+// the share of its tiles that lies inside the result, times the share of the last round of
+// workgroups that is taken.  A chip that is not half full is filled with slices, none
+// shorter than 8 steps, if the results may be partial sums.
+inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, bool may_slice) {
+  Cut best{false, 1};
+  double best_score = -1.0;
+  for (int large = 0; large < 2; ++large) {
+    const int64_t side = large ? 256 : 128, room = large ? 256 : 512;
+    const int64_t tq = tiles_along(rows_q, side), tp = tiles_along(rows_p, side);
+    int64_t slices = may_slice ? room / (tq * tp) : 1;
+    if (slices > steps / 8) slices = steps / 8;
+    if (slices < 1) slices = 1;
+    const int64_t groups = tq * tp * slices;
+    const double inside = (double)rows_q * (double)rows_p / ((double)(tq * tp) * (double)(side * side));
+    const double taken = (double)groups / ((double)tiles_along(groups, room) * (double)room);
+    const double score = inside * taken * (large ? 1.2 : 1.0);
+    if (score > best_score) {
+      best_score = score;
+      best = Cut{large != 0, (int)slices};
+    }
+  }
+  return best;
 }
 
 template <class T, class E>
@@ -358,11 +787,24 @@ int launch_tiles(Problem pr, int slices, const E& epilogue, hipStream_t stream) 
   return launch_status();
 }
 
-// A tile's rows, and the offsets inside it, have to fit the buffer descriptor.
-inline bool operand_fits(const Operand& o, int64_t k_bytes) {
-  return o.ld > 0 && o.ld <= (1 << 22) && k_bytes <= o.ld && o.ld % 16 == 0 &&
-         aligned_to(o.base, 16) && k_bytes % 16 == 0;
+template <class T, bool KQ, bool KP, class E>
+int launch_product(const Problem& pr, const Cut& cut, const E& epilogue, hipStream_t stream) {
+  return cut.large ? launch_tiles<Large<T, KQ, KP>, E>(pr, cut.slices, epilogue, stream)
+                   : launch_tiles<Small<T, KQ, KP>, E>(pr, cut.slices, epilogue, stream);
 }
+
+// Carves a workspace; with a null base it only counts.
+inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+struct Carver {
+  uint8_t* base;
+  size_t used = 0;
+  template <class P>
+  P* take(int64_t count) {
+    P* p = reinterpret_cast<P*>(base ? base + used : nullptr);
+    used += (size_t)up_to(count * (int64_t)sizeof(P), 256);
+    return p;
+  }
+};
 
 }  // namespace gemm
 }  // namespace oa

@@ -62,10 +62,12 @@ def _expected(x, w, y, grad, reduction, ignore_index=-100):
     dx_tol = (up_abs * ((err + d.abs() * (v + 8) * 2 * U) @ w.abs())) + dx.abs() * r
     e = err * up_abs + 2.0**-126
     if r == 2.0**-11:
+        # d under its lift, and x times a power of two: fp16's smallest step is 2^-24
         e = e + 2.0**-40 * up.abs().max()
+        small_x = 2.0**-25 * d.abs().sum(0)[:, None] * up.abs().max()
     dw = (d * up[:, None]).t().contiguous() @ x
     dw_tol = (e + (d * up[:, None]).abs() * (t + 8) * 2 * U).t().contiguous() @ x.abs()
-    dw_tol = dw_tol + dw.abs() * r
+    dw_tol = dw_tol + dw.abs() * r + (small_x if r == 2.0**-11 else 0.0)
     tiny = torch.finfo(torch.float16).smallest_normal * 2.0**-10 if r == 2.0**-11 else 0.0
     return (loss, loss_tol), (dx, dx_tol + tiny), (dw, dw_tol + tiny)
 
