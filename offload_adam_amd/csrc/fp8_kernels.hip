@@ -203,36 +203,6 @@ fp8_decode_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sca
   }
 }
 
-// Codes [rows][cols] -> [cols][ld_out], zeros for rows up to ld_out.
-__global__ void __launch_bounds__(kThreads)
-fp8_transpose_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int64_t blocks_c,
-                     uint8_t* __restrict__ out, int64_t ld_out) {
-  __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];  // [column][row]
-  const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
-  const int r = threadIdx.x / 16 * kPatch, c = threadIdx.x % 16 * kPatch;
-  const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
-  u32x2 w[kPatch];
-#pragma unroll
-  for (int p = 0; p < kPatch; ++p)
-    w[p] = r0 + p < rows && c0 < cols ? *reinterpret_cast<const u32x2*>(q + (r0 + p) * cols + c0)
-                                      : u32x2{0u, 0u};
-#pragma unroll
-  for (int j = 0; j < kPatch; ++j) {
-    u8x8 o;
-#pragma unroll
-    for (int p = 0; p < kPatch; ++p) o[p] = (uint8_t)(w[p][j / 4] >> (8 * (j % 4)));
-    *reinterpret_cast<u8x8*>(&tile[c + j][r]) = o;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int i = threadIdx.x + kThreads * k, col = i / 8, piece = i % 8 * 16;
-    if (bc * kBlock + col < cols)
-      *reinterpret_cast<u32x4*>(out + (bc * kBlock + col) * ld_out + br * kBlock + piece) =
-          *reinterpret_cast<const u32x4*>(&tile[col][piece]);
-  }
-}
-
 // ----------------------------------------------------------- operand encoder
 
 // A matrix [rows][cols] as operands of the products, in one read of it:
@@ -330,6 +300,40 @@ fp8_operand_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, i
   }
 }
 
+// The row operand alone (codes in blocks of 1 x 128 along the columns): 16 lanes to a
+// block, eight elements to a lane, columns from `cols` up to e.ld zero.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+fp8_rows_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols, bool vec,
+                const Encoded e) {
+  const int64_t per_row = e.ld / kPatch;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t r = i / per_row, c = i % per_row * kPatch;
+  if (r >= rows) return;  // 16 lanes together: rows are whole blocks long
+  float x[kPatch] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  if (vec) {
+    if (c < cols) load8<DT>(src, r * stride + c, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j)
+      if (c + j < cols) x[j] = load1<DT>(src, r * stride + c + j);
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < kPatch; ++j) {
+    if (fabsf(x[j]) == INFINITY) x[j] = NAN;
+    top = fmaxf(top, fabsf(x[j]));
+  }
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+  const uint32_t s = scale_of(top);
+  const float down = down_of(s);
+  *reinterpret_cast<u32x2*>(e.q + r * e.ld + c) =
+      u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
+            encode4(x[4] * down, x[5] * down, x[6] * down, x[7] * down)};
+  if (threadIdx.x % 16 == 0) e.scales[packed_scale_at(r, c / kBlock, e.scale_stride)] = (uint8_t)s;
+}
+
 // Column sums: the row blocks' sums in order.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
@@ -410,6 +414,85 @@ struct SliceEpilogue {
   }
 };
 
+// ---- few tokens.  Bound by reading the weight once.  A workgroup of eight waves makes 16
+// columns of y; each wave takes every eighth step of k, its fragments straight from
+// memory to registers (16 rows of 128 bytes each, four steps ahead of the products, so that
+// the loads of all waves of a CU cover the latency), multiplies them with all the tokens,
+// up to four tiles of 16, and the waves' sums meet in LDS, in order.
+constexpr int kFewWaves = 8, kFewAhead = 4;
+
+template <int DT, int TILES>
+__global__ void __launch_bounds__(kFewWaves* kWave)
+fp8_few_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, int64_t out_f,
+               int in_f, int blocks_k, const uint8_t* __restrict__ xq,
+               const uint8_t* __restrict__ xs, int64_t ldx, int64_t xs_stride, int tokens,
+               const void* __restrict__ bias, void* __restrict__ y) {
+  __shared__ __align__(16) float sums[kFewWaves][TILES][kLines][kLines + 4];  // [token][column]
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t n0 = (int64_t)blockIdx.x * kLines;
+  const int r = lane % kLines, k0 = lane / kLines * 32;
+  const int64_t n = n0 + r < out_f ? n0 + r : out_f - 1;  // rows past the end: not stored
+  const uint8_t* wrow = w + n * in_f + k0;
+  const uint8_t* scale = ws + n0 / kBlock * blocks_k;
+  f32x4 acc[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto fetch = [&](int step, i32x8& q, int& sq) {
+    const int k = step * kStepBytes + k0;
+    i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    sq = 0;
+    if (step < blocks_k) {
+      if (k < in_f) lo = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes);
+      if (k + 16 < in_f) hi = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes + 16);
+      sq = scale[step];
+    }
+    q = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  i32x8 q[kFewAhead];
+  int sq[kFewAhead];
+#pragma unroll
+  for (int i = 0; i < kFewAhead; ++i) fetch(wave + i * kFewWaves, q[i], sq[i]);
+  for (int step = wave; step < blocks_k; step += kFewAhead * kFewWaves) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int at = step + i * kFewWaves;
+      if (at < blocks_k) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          const int token = t * kLines + r;
+          i32x8 p = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (token < tokens) {  // rows of codes are whole steps long
+            const uint8_t* x = xq + token * ldx + at * kStepBytes + k0;
+            p = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(x),
+                                        *reinterpret_cast<const i32x4*>(x + 16), 0, 1, 2, 3, 4, 5,
+                                        6, 7);
+          }
+          const int sp = token < tokens ? xs[packed_scale_at(token, at, xs_stride)] : 0;
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[i], p, acc[t], 0, 0, 0,
+                                                                    sq[i], 0, sp);
+        }
+      }
+      fetch(at + kFewAhead * kFewWaves, q[i], sq[i]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    asm volatile("" : "+v"(acc[t]));  // here, on every lane
+    *reinterpret_cast<f32x4*>(&sums[wave][t][r][lane / kLines * 4]) = acc[t];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TILES * kLines * kLines; i += kFewWaves * kWave) {
+    const int token = i / kLines, c = i % kLines;
+    if (token >= tokens || n0 + c >= out_f) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kFewWaves; ++g) v += sums[g][token / kLines][token % kLines][c];
+    if (bias) v += load1<DT>(bias, n0 + c);
+    store1<DT>(y, token * out_f + n0 + c, v);
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 fp8_join_kernel(const float* __restrict__ part, int slices, int64_t count, int64_t cols,
@@ -434,15 +517,15 @@ struct Output {
   }
 };
 
-template <int DT, bool Q_PACKED>
+template <int DT, bool Q_PACKED, bool Q_LINES>
 int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hipStream_t s) {
   typedef E4m3<Q_PACKED> T;
   if (o.cut.slices == 1) {
     const StoreEpilogue<DT> e{out, o.rows, o.cols, bias, o.cols % 8 == 0 && aligned_to(out, 16)};
-    return launch_product<T, false, false>(pr, o.cut, e, s);
+    return launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
   }
   const SliceEpilogue e{o.part, o.rows, o.cols, o.cols % 4 == 0};
-  int rc = launch_product<T, false, false>(pr, o.cut, e, s);
+  int rc = launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
   if (rc) return rc;
   const int64_t count = o.rows * o.cols;
   hipLaunchKernelGGL(fp8_join_kernel<DT>, dim3((unsigned)((count + kThreads - 1) / kThreads)),
@@ -468,6 +551,18 @@ int encode_operand(const Source& m, const Encoded& e, hipStream_t s) {
   return launch_status();
 }
 
+template <int DT>
+int encode_rows(const Source& m, const Encoded& e, hipStream_t s) {
+  const int64_t lanes = m.rows * (e.ld / kPatch);
+  hipLaunchKernelGGL(fp8_rows_kernel<DT>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)),
+                     dim3(kThreads), 0, s, m.base, m.stride, m.rows, m.cols, vector_rows(m, DT), e);
+  return launch_status();
+}
+
+// Up to this many tokens the weight's bytes are what the product takes; a tile of 128
+// tokens in slices took 14 + 4 us where 58 MB can be read in 11.
+constexpr int64_t kFewTokens = 64;
+
 struct Layer {
   const uint8_t *q, *scales;
   int64_t out_f, in_f;
@@ -483,7 +578,7 @@ struct ForwardPlan {
     x.scale_stride = up_to(tokens, 256);
     x.q = c.take<uint8_t>(tokens * x.ld);
     x.scales = c.take<uint8_t>(blocks_of(in_f) * x.scale_stride);
-    y = Output(tokens, out_f, in_f, c);
+    if (tokens > kFewTokens) y = Output(tokens, out_f, in_f, c);
     bytes = c.used;
   }
 };
@@ -491,20 +586,40 @@ struct ForwardPlan {
 template <int DT>
 int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws, hipStream_t s) {
   const ForwardPlan plan(x.rows, w.in_f, w.out_f, ws);
-  int rc = encode_operand<DT>(x, plan.x, s);
+  int rc = encode_rows<DT>(x, plan.x, s);
   if (rc) return rc;
+  if (x.rows <= kFewTokens) {
+    const dim3 grid((unsigned)tiles_along(w.out_f, kLines)), block(kFewWaves * kWave);
+    const int blocks = (int)blocks_of(w.in_f), tokens = (int)x.rows;
+    switch (tiles_along(x.rows, kLines)) {
+      case 1:
+        hipLaunchKernelGGL((fp8_few_kernel<DT, 1>), grid, block, 0, s, w.q, w.scales, w.out_f,
+                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
+                           plan.x.scale_stride, tokens, bias, y);
+        break;
+      case 2:
+        hipLaunchKernelGGL((fp8_few_kernel<DT, 2>), grid, block, 0, s, w.q, w.scales, w.out_f,
+                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
+                           plan.x.scale_stride, tokens, bias, y);
+        break;
+      default:
+        hipLaunchKernelGGL((fp8_few_kernel<DT, 4>), grid, block, 0, s, w.q, w.scales, w.out_f,
+                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
+                           plan.x.scale_stride, tokens, bias, y);
+    }
+    return launch_status();
+  }
   Problem pr{};
   pr.q = Operand{w.q, w.in_f, w.out_f, 0};
   pr.p = Operand{plan.x.q, plan.x.ld, x.rows, 0};
   pr.sq = Scales{w.scales, 1, blocks_of(w.in_f), blocks_of(w.out_f)};
   pr.sp = Scales{plan.x.scales, plan.x.scale_stride, 0, 0};
   pr.k_bytes = (int)w.in_f;
-  return multiply<DT, false>(pr, plan.y, bias, y, s);
+  return multiply<DT, false, false>(pr, plan.y, bias, y, s);
 }
 
 struct BackwardPlan {
   Encoded g{}, x{};
-  uint8_t* wt = nullptr;
   Output dx, dw;
   size_t bytes;
   BackwardPlan(int64_t tokens, int64_t in_f, int64_t out_f, bool want_dx, bool want_dw,
@@ -516,7 +631,6 @@ struct BackwardPlan {
       g.scale_stride = up_to(tokens, 256);
       g.q = c.take<uint8_t>(tokens * g.ld);
       g.scales = c.take<uint8_t>(blocks_of(out_f) * g.scale_stride);
-      wt = c.take<uint8_t>(in_f * padded_n);
       dx = Output(tokens, in_f, padded_n, c);
     }
     if (want_dw) {
@@ -541,18 +655,15 @@ int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* d
   int rc = encode_operand<DT>(g, plan.g, s);
   if (rc) return rc;
   if (dx) {
-    const int64_t bc = blocks_of(w.in_f), br = blocks_of(w.out_f);
-    hipLaunchKernelGGL(fp8_transpose_kernel, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s, w.q,
-                       w.out_f, w.in_f, bc, plan.wt, plan.g.ld);
-    rc = launch_status();
-    if (rc) return rc;
+    // the weight as it lies: line by line along the outputs, which are summed over
+    const int64_t bc = blocks_of(w.in_f);
     Problem pr{};
-    pr.q = Operand{plan.wt, plan.g.ld, w.in_f, 0};
+    pr.q = Operand{w.q, w.in_f, w.in_f, w.out_f};
     pr.p = Operand{plan.g.q, plan.g.ld, g.rows, 0};
     pr.sq = Scales{w.scales, bc, 1, bc};
     pr.sp = Scales{plan.g.scales, plan.g.scale_stride, 0, 0};
     pr.k_bytes = (int)plan.g.ld;
-    rc = multiply<DT, false>(pr, plan.dx, nullptr, dx, s);
+    rc = multiply<DT, false, true>(pr, plan.dx, nullptr, dx, s);
     if (rc) return rc;
   }
   if (dw) {
@@ -564,7 +675,7 @@ int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* d
     pr.sq = Scales{plan.x.scales_t, plan.x.scale_stride_t, 0, 0};
     pr.sp = Scales{plan.g.scales_t, plan.g.scale_stride_t, 0, 0};
     pr.k_bytes = (int)plan.x.ld_t;
-    rc = multiply<DT, true>(pr, plan.dw, nullptr, dw, s);
+    rc = multiply<DT, true, false>(pr, plan.dw, nullptr, dw, s);
     if (rc) return rc;
   }
   if (db) {

@@ -395,8 +395,8 @@ struct ForwardPlan {
   float *z_target, *block_sum;
   int* block_count;
   size_t bytes;
-  ForwardPlan(int64_t tokens, int64_t vocab, void* ws) {
-    cut = cut_for(vocab, tokens > 0 ? tokens : 1, 0, false);
+  ForwardPlan(int64_t tokens, int64_t hidden, int64_t vocab, void* ws) {
+    cut = cut_for(vocab, tokens > 0 ? tokens : 1, steps_of(hidden * 2), false);
     tiles = (int)tiles_along(vocab, cut.large ? 256 : 128);
     blocks = (int)tiles_along(tokens, kCombineTokens);
     Carver c{static_cast<uint8_t*>(ws)};
@@ -456,7 +456,7 @@ Problem logits_problem(const Head& h, int64_t first, int64_t rows) {
 template <class T>
 int forward(const Head& h, int reduction, float* loss, float* lse, float* count, void* ws,
             hipStream_t s) {
-  const ForwardPlan plan(h.tokens, h.vocab, ws);
+  const ForwardPlan plan(h.tokens, h.hidden, h.vocab, ws);
   if (h.tokens > 0) {
     const StatsEpilogue e{h.target, h.tokens, h.vocab, plan.part, plan.z_target};
     int rc = launch_product<T, false, false>(logits_problem(h, 0, h.vocab), plan.cut, e, s);
@@ -495,7 +495,8 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
     const int64_t rows = h.vocab - first < plan.piece ? h.vocab - first : plan.piece;
     const ProbEpilogue<T> pe{h.target, lse, f.d, h.tokens, rows, first, plan.d, plan.piece};
     rc = launch_product<T, false, false>(logits_problem(h, first, rows),
-                                         cut_for(rows, h.tokens, 0, false), pe, s);
+                                         cut_for(rows, h.tokens, steps_of(h.hidden * 2), false), pe,
+                                         s);
     if (rc) return rc;
     if (dx) {
       Problem px{};
@@ -512,7 +513,8 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
       pw.p = Operand{reinterpret_cast<uint8_t*>(plan.d), plan.piece * 2, rows, h.tokens};
       pw.k_bytes = (int)(up_to(h.tokens, 8) * 2);
       const WeightGradEpilogue<T> we{dw + first * h.hidden, rows, h.hidden, f.dw};
-      rc = launch_product<T, true, true>(pw, cut_for(h.hidden, rows, 0, false), we, s);
+      rc = launch_product<T, true, true>(
+          pw, cut_for(h.hidden, rows, steps_of(pw.k_bytes), false), we, s);
       if (rc) return rc;
     }
   }
@@ -549,7 +551,7 @@ extern "C" size_t oa_linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, i
                                                int backward, int want_dx, int want_dw) {
   if (tokens < 0 || hidden <= 0 || vocab <= 0) return 0;
   // never 0: the workspace of an empty batch is a valid pointer too
-  if (!backward) return ForwardPlan(tokens, vocab, nullptr).bytes + 256;
+  if (!backward) return ForwardPlan(tokens, hidden, vocab, nullptr).bytes + 256;
   if (tokens == 0) return 0;
   return BackwardPlan(tokens, hidden, vocab, want_dx != 0, want_dw != 0, nullptr).bytes;
 }

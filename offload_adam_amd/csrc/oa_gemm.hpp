@@ -140,8 +140,8 @@ struct E4m3 {
 };
 
 // An operand: rows of `ld` bytes (16-byte aligned), k_bytes of each taking part (a
-// multiple of 16); or, of 16-bit types, the other way round: `lines` lines of `ld` bytes,
-// one for each k, that hold one element of every row.
+// multiple of 16); or, the other way round, `lines` lines of `ld` bytes, one for each k,
+// that hold one element of every row (whole 16-byte chunks of them).
 struct Operand {
   const uint8_t* base;
   int64_t ld;
@@ -201,14 +201,17 @@ __device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_p, uint32_t t
   tq = in / wide;
 }
 
-// KQ, KP: the operand lies line by line.  Its units are then lines of R elements, 64 of
-// them, and LDS hands the fragments out transposed (a lane gets four k of its row).  Tile t
-// (32 bytes) of a line sits at position t ^ f(line), which puts the lines that are read
-// together into different banks.
+// KQ, KP: the operand lies line by line.  Its units are then lines of R elements, as many
+// as a step has k, and LDS hands the fragments out transposed (a lane gets four 16-bit or
+// eight 8-bit k of its row).  Tile t of a line (16 elements) sits at position t ^ f(line),
+// which puts the lines that are read together into different banks.
 template <class T, int B, bool KQ = false, bool KP = false>
 struct Tile {
   typedef T Type;
-  static_assert(!T::kScaled || (!KQ && !KP), "8-bit operands lie row by row");
+  static_assert(!T::kScaled || (!T::kQPacked && !KP) || (!KQ && !KP),
+                "scales of an operand that lies line by line are per block");
+  static constexpr int kBytes = T::kScaled ? 1 : 2;         // of an element
+  static constexpr int kStepLines = kStepBytes / kBytes;    // k elements of a step
   static constexpr int BQ = B, BP = B;
   static constexpr int kWavesQ = 2, kWaves = 4, kThreads = kWave * kWaves;
   static constexpr int R = B / 2;        // rows of either operand that a wave multiplies: a unit
@@ -255,8 +258,10 @@ struct Tile {
   int at[2];  // where this lane's chunks of the lower and the upper 64 bytes are in a unit
   // ... and of an operand that lies line by line: where its piece of tile t of its line is
   int at_line[N];
-  static constexpr int kLineBytes = R * 2;
+  static constexpr int kLineBytes = R * kBytes, kLineTile = 16 * kBytes;
   static __device__ __forceinline__ int line_swizzle(int line) {
+    if (T::kScaled)
+      return R == 128 ? (line >> 1 & 3) | (line >> 4 & 1) << 2 : (line >> 2 & 1) | (line >> 4 & 1) << 1;
     return R == 128 ? (line & 3) | (line >> 3 & 1) << 2 : (line >> 1 & 1) | (line >> 3 & 1) << 1;
   }
 
@@ -278,24 +283,39 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[4 * I + i] = v[i];
   }
-  // Four k of this lane's row, from the pieces that the 16 lanes of its group point to.
+  // Eight bytes of k of this lane's row, from the pieces that the 16 lanes of its group
+  // point to.
   template <int I>
   static __device__ __forceinline__ void put_lines(typename T::Frag& f, const uint8_t* src) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef int i32x2 __attribute__((ext_vector_type(2)));
-    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4*)(const_cast<uint8_t*>(src)));
-    const i32x2 w = __builtin_bit_cast(i32x2, v);
+    i32x2 w;
+    if constexpr (T::kScaled)
+      w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (__attribute__((address_space(3))) i32x2*)(const_cast<uint8_t*>(src)));
+    else
+      w = __builtin_bit_cast(
+          i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     (__attribute__((address_space(3))) s16x4*)(const_cast<uint8_t*>(src))));
     f[2 * I] = w[0];
     f[2 * I + 1] = w[1];
   }
+  // Lines from one read of a tile to the next: 16-bit, half HALF, reads 0 and 1; 8-bit, four
+  // reads of both 64-byte parts.
+  static constexpr int line_ahead(int half, int i) {
+    return T::kScaled ? 64 * (i / 2) + 8 * (i % 2) : 32 * half + 4 * i;
+  }
   // Fragments of half HALF, reads I ... of q's and of p's.
-  static constexpr int kReadsQ = KQ ? 2 * N : H * kPieces, kReadsP = KP ? 2 * N : N * kPieces;
+  static constexpr int kLineReads = 2 * kPieces;
+  static constexpr int kReadsQ = H * (KQ ? kLineReads : kPieces);
+  static constexpr int kReadsP = N * (KP ? kLineReads : kPieces);
   template <int HALF, int I, int COUNT>
   __device__ __forceinline__ void read_q(const From& r, Fragments& f) const {
     if constexpr (COUNT > 0) {
       if constexpr (KQ) {
-        put_lines<I % 2>(f.q[HALF][I / 2], r.q[I / 2] + (32 * HALF + 4 * (I % 2)) * kLineBytes);
+        constexpr int t = I / kLineReads, c = I % kLineReads;
+        put_lines<c>(f.q[HALF][t], r.q[t + (kHalvesOfK ? 0 : HALF * H)] +
+                                       line_ahead(HALF, c) * kLineBytes);
       } else {
         constexpr int t = I / kPieces, c = I % kPieces;
         put<c>(f.q[HALF][t], r.q[c], (t + (kHalvesOfK ? 0 : HALF * H)) * kLines);
@@ -307,7 +327,8 @@ struct Tile {
   __device__ __forceinline__ void read_p(const From& r, Fragments& f) const {
     if constexpr (COUNT > 0) {
       if constexpr (KP) {
-        put_lines<I % 2>(f.p[HALF][I / 2], r.p[I / 2] + (32 * HALF + 4 * (I % 2)) * kLineBytes);
+        constexpr int t = I / kLineReads, c = I % kLineReads;
+        put_lines<c>(f.p[HALF][t], r.p[t] + line_ahead(HALF, c) * kLineBytes);
       } else {
         constexpr int t = I / kPieces, c = I % kPieces;
         put<c>(f.p[kHalvesOfK ? HALF : 0][t], r.p[c], t * kLines);
@@ -393,7 +414,7 @@ struct Tile {
     constexpr int o = operand_of<I>(), i = I % kLoads;
     const int offset = w.offset[o][I % (2 * kLoads)];
     if (FULL) return offset;
-    if (o == 0 ? KQ : KP) return step * 64 + line_of(i) < w.lines ? offset : kOut;
+    if (o == 0 ? KQ : KP) return step * kStepLines + line_of(i) < w.lines ? offset : kOut;
     return step * kStepBytes + chunk_of(i) * 16 < w.k_end ? offset : kOut;
   }
   // Load i of a unit that lies line by line: this lane's line.
@@ -404,14 +425,15 @@ struct Tile {
   template <bool LINES>
   __device__ __forceinline__ void start(Walk& w, int o, const Operand& op, int64_t row0, int step0) {
     if constexpr (LINES) {
-      w.rsrc[o] = descriptor(op.base + (int64_t)step0 * 64 * op.ld + row0 * 2, 64 * (int)op.ld);
-      w.step_bytes[o] = 64 * (int)op.ld;
+      w.step_bytes[o] = kStepLines * (int)op.ld;
+      w.rsrc[o] = descriptor(op.base + (int64_t)step0 * w.step_bytes[o] + row0 * kBytes,
+                             w.step_bytes[o]);
 #pragma unroll
       for (int i = 0; i < 2 * kLoads; ++i) {
         const int line = line_of(i % kLoads);
-        const int c = lane % (kLineBytes / 16) ^ 2 * line_swizzle(line);
-        const int row = i / kLoads * R + c * 8;
-        w.offset[o][i] = row0 + row < op.rows ? line * (int)op.ld + row * 2 : kOut;
+        const int c = lane % (kLineBytes / 16) ^ kLineTile / 16 * line_swizzle(line);
+        const int row = i / kLoads * R + c * 16 / kBytes;
+        w.offset[o][i] = row0 + row < op.rows ? line * (int)op.ld + row * kBytes : kOut;
       }
     } else {
       w.rsrc[o] = tile_rsrc(op, row0, B, (int64_t)step0 * kStepBytes);
@@ -651,10 +673,10 @@ struct Tile {
     start<KP>(w, 1, op, row_p, step0);
     w.k_end = k_bytes < step1 * kStepBytes ? k_bytes : step1 * kStepBytes;
     int full = w.k_end / kStepBytes;  // steps that are wholly there
-    w.lines = step1 * 64;
+    w.lines = step1 * kStepLines;
     if (KQ && oq.lines < w.lines) w.lines = (int)oq.lines;
     if (KP && op.lines < w.lines) w.lines = (int)op.lines;
-    if ((KQ || KP) && w.lines / 64 < full) full = w.lines / 64;
+    if ((KQ || KP) && w.lines / kStepLines < full) full = w.lines / kStepLines;
     w.last = step1 - 1;
     w.sq = scq;
     w.sp = scp;
@@ -662,10 +684,12 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       at[i] = lane % kLines * kStepBytes + ((lane / kLines + 4 * i) ^ (lane / 2 % 8)) * 16;
-    const int line = lane / kLines * 8 + lane % kLines / 4;
+    const int line = T::kScaled ? lane / kLines * 16 + lane % kLines / 2
+                                : lane / kLines * 8 + lane % kLines / 4;
 #pragma unroll
     for (int t = 0; t < N; ++t)
-      at_line[t] = line * kLineBytes + (t ^ line_swizzle(line)) * 32 + lane % 4 * 8;
+      at_line[t] = line * kLineBytes + (t ^ line_swizzle(line)) * kLineTile +
+                   lane % (kLineTile / 8) * 8;
 
     const uint32_t base = __builtin_amdgcn_readfirstlane(
         (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
@@ -749,26 +773,31 @@ struct Cut {
   int slices;
 };
 
-// Whichever of the two tiles leaves less of the chip idle, the large one counted 1.2-fold:
-// the share of its tiles that lies inside the result, times the share of the last round of
-// workgroups that is taken.  A chip that is not half full is filled with slices, none
-// shorter than 8 steps, if the results may be partial sums.
+// The cut with the least estimated time, in microseconds: rounds of workgroups times (steps
+// of a slice times the time of one, plus what a tile costs besides), and the traffic of
+// partial results.  Measured with both element types: 1.4 to 1.7 a step and 7 besides for
+// the large tile, 1.0 and 2 for a round of small ones; partial sums move at some 4 TB/s.
+// e4m3, 4096 x 5632 x 2048: 52 us small (54 estimated), 62 estimated large; 4096 x 2048 x
+// 5632: 46 + 16 large in two slices, 46 estimated small; 4096 x 14336 x 4096: 211 large,
+// 270 small; bf16, 4096 x 2048 x 16384: 190 large in two slices, 260 small.
 inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, bool may_slice) {
   Cut best{false, 1};
-  double best_score = -1.0;
+  double least = 0.0;
   for (int large = 0; large < 2; ++large) {
     const int64_t side = large ? 256 : 128, room = large ? 256 : 512;
-    const int64_t tq = tiles_along(rows_q, side), tp = tiles_along(rows_p, side);
-    int64_t slices = may_slice ? room / (tq * tp) : 1;
-    if (slices > steps / 8) slices = steps / 8;
-    if (slices < 1) slices = 1;
-    const int64_t groups = tq * tp * slices;
-    const double inside = (double)rows_q * (double)rows_p / ((double)(tq * tp) * (double)(side * side));
-    const double taken = (double)groups / ((double)tiles_along(groups, room) * (double)room);
-    const double score = inside * taken * (large ? 1.2 : 1.0);
-    if (score > best_score) {
-      best_score = score;
-      best = Cut{large != 0, (int)slices};
+    const double step = large ? 1.5 : 1.0, besides = large ? 7.0 : 2.0;
+    const int64_t tiles = tiles_along(rows_q, side) * tiles_along(rows_p, side);
+    int64_t most = may_slice ? room / tiles : 1;  // a full chip is not cut further
+    if (most > steps / 4) most = steps / 4;
+    if (most < 1) most = 1;
+    for (int64_t slices = 1; slices <= most; ++slices) {
+      double t = (double)tiles_along(tiles * slices, room) *
+                 ((double)tiles_along(steps, slices) * step + besides);
+      if (slices > 1) t += 5.0 + (double)rows_q * (double)rows_p * 8.0 * (double)slices / 4e6;
+      if (least == 0.0 || t < least) {
+        least = t;
+        best = Cut{large != 0, (int)slices};
+      }
     }
   }
   return best;

@@ -9,8 +9,6 @@ gradients.  The reference has no counterpart: its example's model returns logits
 (examples/e2e_train/train.py).
 """
 
-from ctypes import c_int, c_int64, c_size_t
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -43,16 +41,13 @@ def _plain(weight, dtype):
 def _head_args(x, w, target, ignore_index, reduction):
     x, hidden, ldx = _rows(x, "x")
     w, _, ldw = _rows(w, "weight")
-    args = [_lib.ptr(x), c_int64(ldx), _lib.ptr(w), c_int64(ldw),
-            c_int(_lib.dtype_code(x.dtype)), _lib.ptr(target), c_int64(x.shape[0]),
-            c_int64(hidden), c_int64(w.shape[0]), c_int64(ignore_index),
-            c_int(_REDUCTIONS[reduction])]
+    args = [x.data_ptr(), ldx, w.data_ptr(), ldw, _lib.dtype_code(x.dtype), target.data_ptr(),
+            x.shape[0], hidden, w.shape[0], ignore_index, _REDUCTIONS[reduction]]
     return args, hidden, (x, w)
 
 
 def _workspace(device, tokens, hidden, vocab, backward, dx, dw):
-    nbytes = _lib.load().oa_linear_ce_workspace_bytes(
-        c_int64(tokens), c_int64(hidden), c_int64(vocab), c_int(backward), c_int(dx), c_int(dw))
+    nbytes = _lib.load().oa_linear_ce_workspace_bytes(tokens, hidden, vocab, backward, dx, dw)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
@@ -71,8 +66,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
             if loss.numel():
                 ws = _workspace(dev, tokens, hidden, w.shape[0], 0, 0, 0)
                 code = lib.oa_linear_ce_forward(
-                    *args, _lib.ptr(loss), _lib.ptr(lse), _lib.ptr(count), _lib.ptr(ws),
-                    c_size_t(ws.numel()), _lib.current_stream_ptr())
+                    *args, loss.data_ptr(), lse.data_ptr(), count.data_ptr(), ws.data_ptr(),
+                    ws.numel(), _lib.current_stream_ptr())
                 _lib.check(code, "oa_linear_ce_forward")
         ctx.save_for_backward(x, weight, target, lse, count)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
@@ -98,8 +93,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
             dw = torch.empty((vocab, hidden), dtype=x.dtype, device=dev) if want_dw else None
             ws = _workspace(dev, tokens, hidden, vocab, 1, int(want_dx), int(want_dw))
             code = lib.oa_linear_ce_backward(
-                *args, _lib.ptr(lse), _lib.ptr(count), _lib.ptr(grad), _lib.ptr(dx),
-                _lib.ptr(dw), _lib.ptr(ws), c_size_t(ws.numel()), _lib.current_stream_ptr())
+                *args, lse.data_ptr(), count.data_ptr(), grad.data_ptr(),
+                dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dw else None,
+                ws.data_ptr(), ws.numel(), _lib.current_stream_ptr())
             _lib.check(code, "oa_linear_ce_backward")
             if hidden != x.shape[1]:  # operands were padded
                 dx = dx[:, :x.shape[1]].contiguous() if want_dx else None

@@ -3,7 +3,7 @@ fresh (or given) tensor.  GPU tensors only; every function enqueues on the
 current stream of the tensor's device and returns without synchronising.
 """
 
-from ctypes import c_int, c_int64, c_size_t
+from ctypes import c_int, c_int64
 
 import torch
 
@@ -184,28 +184,31 @@ def _fp8_payload(codes, scale):
     return rows, cols
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def quantize_fp8_into(src, codes, scale):
     src, stride = _rows_view(src)
     rows, cols = _fp8_payload(codes, scale)
     if tuple(src.shape) != (rows, cols) or src.device != codes.device:
         raise ValueError(f"cannot encode {tuple(src.shape)} on {src.device} into a "
                          f"{rows} x {cols} weight on {codes.device}")
-    _call("oa_quant_fp8", src.device, _lib.ptr(src), c_int(_lib.dtype_code(src.dtype)),
-          c_int64(stride), c_int64(rows), c_int64(cols), _lib.ptr(codes), _lib.ptr(scale))
+    _call("oa_quant_fp8", src.device, src.data_ptr(), _lib.dtype_code(src.dtype), stride, rows,
+          cols, codes.data_ptr(), scale.data_ptr())
     mark_written(codes, scale)
 
 
 def dequantize_fp8(codes, scale, out_dtype):
     rows, cols = _fp8_payload(codes, scale)
     out = torch.empty((rows, cols), dtype=out_dtype, device=codes.device)
-    _call("oa_dequant_fp8", codes.device, _lib.ptr(codes), _lib.ptr(scale), c_int64(rows),
-          c_int64(cols), _lib.ptr(out), c_int(_lib.dtype_code(out_dtype)), c_int64(max(cols, 1)))
+    _call("oa_dequant_fp8", codes.device, codes.data_ptr(), scale.data_ptr(), rows, cols,
+          out.data_ptr(), _lib.dtype_code(out_dtype), max(cols, 1))
     return out
 
 
 def _fp8_workspace(device, *sizes):
-    nbytes = _lib.load().oa_fp8_linear_workspace_bytes(*[c_int64(v) for v in sizes[:3]],
-                                                       *[c_int(v) for v in sizes[3:]])
+    nbytes = _lib.load().oa_fp8_linear_workspace_bytes(*sizes)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
@@ -213,15 +216,14 @@ def fp8_linear_forward(x, codes, scale, bias):
     """x (T, in) -> (T, out) in x's dtype."""
     x, ldx = _rows_view(x)
     out_f, in_f = _fp8_payload(codes, scale)
-    dt = c_int(_lib.dtype_code(x.dtype))
+    dt = _lib.dtype_code(x.dtype)
     tokens, dev = x.shape[0], x.device
     y = torch.empty((tokens, out_f), dtype=x.dtype, device=dev)
     if y.numel() == 0:
         return y
     ws = _fp8_workspace(dev, tokens, in_f, out_f, 0, 0, 0, 0)
-    _call("oa_fp8_linear_forward", dev, _lib.ptr(x), c_int64(ldx), dt, c_int64(tokens),
-          _lib.ptr(codes), _lib.ptr(scale), _lib.ptr(bias), c_int64(out_f), c_int64(in_f),
-          _lib.ptr(y), _lib.ptr(ws), c_size_t(ws.numel()))
+    _call("oa_fp8_linear_forward", dev, x.data_ptr(), ldx, dt, tokens, codes.data_ptr(),
+          scale.data_ptr(), _addr(bias), out_f, in_f, y.data_ptr(), ws.data_ptr(), ws.numel())
     return y
 
 
@@ -230,7 +232,7 @@ def fp8_linear_backward(grad, x, codes, scale, want_dx, want_dw, want_db):
     grad, ldg = _rows_view(grad)
     x, ldx = _rows_view(x)
     out_f, in_f = _fp8_payload(codes, scale)
-    dt = c_int(_lib.dtype_code(x.dtype))
+    dt = _lib.dtype_code(x.dtype)
     tokens, dev = x.shape[0], x.device
     make = torch.empty if tokens and out_f else torch.zeros
     dx = make((tokens, in_f), dtype=x.dtype, device=dev) if want_dx else None
@@ -238,8 +240,7 @@ def fp8_linear_backward(grad, x, codes, scale, want_dx, want_dw, want_db):
     db = make((out_f,), dtype=x.dtype, device=dev) if want_db else None
     if tokens and out_f and (want_dx or want_dw or want_db):
         ws = _fp8_workspace(dev, tokens, in_f, out_f, 1, int(want_dx), int(want_dw), int(want_db))
-        _call("oa_fp8_linear_backward", dev, _lib.ptr(grad), c_int64(ldg), _lib.ptr(x),
-              c_int64(ldx), dt, c_int64(tokens), _lib.ptr(codes), _lib.ptr(scale),
-              c_int64(out_f), c_int64(in_f), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
-              _lib.ptr(ws), c_size_t(ws.numel()))
+        _call("oa_fp8_linear_backward", dev, grad.data_ptr(), ldg, x.data_ptr(), ldx, dt, tokens,
+              codes.data_ptr(), scale.data_ptr(), out_f, in_f, _addr(dx), _addr(dw), _addr(db),
+              ws.data_ptr(), ws.numel())
     return dx, dw, db

@@ -99,6 +99,16 @@ def _quantize_fp8_hip(tensor):
     return weight, scale
 
 
+def _linear_forward(x, weight, bias):
+    flat = x.reshape(-1, x.shape[-1])
+    if x.is_cuda:
+        y = _codec_ops.fp8_linear_forward(flat, weight.weight, weight.block_scale, bias)
+    else:
+        y = _held(flat, 1, FP8_BLOCK) @ weight.dequantize(torch.float32).T
+        y = (y if bias is None else y + bias.float()).to(x.dtype)
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])
+
+
 class _FP8Linear(torch.autograd.Function):
     """GPU operands go to the HIP kernels; CPU operands (model surgery, host tests) take
     the same definition in torch arithmetic."""
@@ -106,13 +116,7 @@ class _FP8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         ctx.save_for_backward(x, weight)
-        flat = x.reshape(-1, x.shape[-1])
-        if x.is_cuda:
-            y = _codec_ops.fp8_linear_forward(flat, weight.weight, weight.block_scale, bias)
-        else:
-            y = _held(flat, 1, FP8_BLOCK) @ weight.dequantize(torch.float32).T
-            y = (y if bias is None else y + bias.float()).to(x.dtype)
-        return y.reshape(*x.shape[:-1], weight.shape[0])
+        return _linear_forward(x, weight, bias)
 
     @staticmethod
     @once_differentiable
@@ -243,6 +247,10 @@ def _linear(func, types, args, kwargs):
                 raise ValueError(f"linear: bias must have shape ({weight.shape[0]},) on "
                                  f"{input.device}, got {tuple(bias.shape)} on {bias.device}")
             bias = bias.to(input.dtype).contiguous()
+        if not torch.is_grad_enabled() or not (
+                input.requires_grad or weight.requires_grad
+                or (bias is not None and bias.requires_grad)):
+            return _linear_forward(input, weight, bias)
         return _FP8Linear.apply(input, weight, bias)
 
     return run(*args, **kwargs)
