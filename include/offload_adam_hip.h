@@ -374,7 +374,8 @@ int oa_adam_requant_nvfp4(const void* grad, void* exp_avg, void* exp_avg_sq,
  *            [0, vocab) makes the token's loss and its gradients NaN
  *   loss     f32: one element (mean over the tokens that take part, NaN if there
  *            are none; or sum), or [tokens] (none)
- *   lse      f32[tokens], count f32[1]: for the backward pass
+ *   lse      f32[tokens], count f32[1]: for the backward pass (count is neither
+ *            written nor read for losses of every token)
  *   workspace  oa_linear_ce_workspace_bytes() bytes, 256-byte aligned, used until
  *            the enqueued work has run
  * Sizes: hidden strides up to 2^20 elements, 2^22 tokens, 2^24 rows of w.

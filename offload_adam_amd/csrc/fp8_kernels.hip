@@ -36,23 +36,36 @@ __device__ __forceinline__ float load1(const void* base, int64_t i) {
   return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
+// Eight elements as they lie in memory.
+template <int DT>
+struct Octet {
+  static constexpr int kWords = DT == OA_F32 ? 2 : 1;
+  u32x4 w[kWords];
+
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(base) +
+                                                    i * (DT == OA_F32 ? 4 : 2));
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = p[k];
+  }
+  __device__ __forceinline__ float operator[](int k) const {
+    if (DT == OA_F32) return __uint_as_float(w[k / 4 % kWords][k % 4]);
+    const uint16_t h = (uint16_t)(w[0][k / 2 % 4] >> (16 * (k % 2)));
+    return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+  }
+  // element k of a row that is loaded piece by piece; the octet starts as zeros
+  __device__ __forceinline__ void put(int k, const void* base, int64_t i) {
+    if (DT == OA_F32) w[k / 4 % kWords][k % 4] = static_cast<const uint32_t*>(base)[i];
+    else w[0][k / 2 % 4] |= (uint32_t)static_cast<const uint16_t*>(base)[i] << (16 * (k % 2));
+  }
+};
+
 template <int DT>
 __device__ __forceinline__ void load8(const void* base, int64_t i, float (&x)[8]) {
-  if (DT == OA_F32) {
-    const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i);
-    const f32x4 a = p[0], b = p[1];
+  Octet<DT> o;
+  o.load(base, i);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = a[k];
-      x[4 + k] = b[k];
-    }
-  } else {
-    const u16x8 w = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(base) + i);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[k] = DT == OA_BF16 ? bf16_bits_to_f32(w[k])
-                           : (float)__builtin_bit_cast(_Float16, (unsigned short)w[k]);
-  }
+  for (int k = 0; k < 8; ++k) x[k] = o[k];
 }
 
 template <int DT>
@@ -414,66 +427,150 @@ struct SliceEpilogue {
   }
 };
 
-// ---- few tokens.  Bound by reading the weight once.  A workgroup of eight waves makes 16
-// columns of y; each wave takes every eighth step of k, its fragments straight from
-// memory to registers (16 rows of 128 bytes each, four steps ahead of the products, so that
-// the loads of all waves of a CU cover the latency), multiplies them with all the tokens,
-// up to four tiles of 16, and the waves' sums meet in LDS, in order.
-constexpr int kFewWaves = 8, kFewAhead = 4;
+struct Source {
+  const void* base;
+  int64_t stride, rows, cols;
+};
 
-template <int DT, int TILES>
-__global__ void __launch_bounds__(kFewWaves* kWave)
-fp8_few_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, int64_t out_f,
-               int in_f, int blocks_k, const uint8_t* __restrict__ xq,
-               const uint8_t* __restrict__ xs, int64_t ldx, int64_t xs_stride, int tokens,
-               const void* __restrict__ bias, void* __restrict__ y) {
-  __shared__ __align__(16) float sums[kFewWaves][TILES][kLines][kLines + 4];  // [token][column]
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+// ---- few tokens.  Bound by reading the weight once.  A workgroup makes 16 columns of y;
+// each of its waves takes every WAVES-th step of k, its fragments straight from memory to
+// registers (16 rows of 128 bytes each), two or four steps ahead of the products, so that the
+// loads of all waves of a CU cover the latency, multiplies them with all the tokens, one or
+// two tiles of 16, and the waves' sums meet in LDS, in order.  ENCODE: x comes as it is
+// and every workgroup makes the codes for itself, in LDS, while its weights are on the way.
+template <int DT>
+struct Few {
+  const uint8_t *w, *ws;
+  int64_t out_f;
+  int in_f, blocks_k;
+  Source x;            // ENCODE
+  bool vec;
+  const uint8_t *xq, *xs;  // else
+  int64_t ldx;         // of the codes
+  int64_t xs_stride;
+  int tokens;
+  const void* bias;
+  void* y;
+};
+
+constexpr int kFewCodes = 16384, kFewEncodeTokens = 16;  // ENCODE: codes, and tokens, at most
+
+template <int DT, int TILES, int WAVES, bool ENCODE>
+__global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) {
+  static_assert(!ENCODE || TILES == 1, "a workgroup encodes the tokens of one tile");
+  constexpr int kLanes = WAVES * kWave;
+  constexpr int kFewAhead = TILES * WAVES >= 32 ? 2 : 4;  // what the registers hold
+  constexpr int kPieces = ENCODE ? kFewCodes / kPatch / kLanes : 1;
+  __shared__ __align__(16) float sums[WAVES][TILES][kLines][kLines + 4];  // [token][column]
+  __shared__ __align__(16) uint8_t codes[ENCODE ? kFewCodes : 16];
+  __shared__ uint8_t scales[ENCODE ? kFewCodes / kBlock : 1];
+  const int lane = threadIdx.x % kWave;
+  // the same in all lanes, and known to be: a matrix instruction does not look at which
+  // lanes are switched off
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t n0 = (int64_t)blockIdx.x * kLines;
   const int r = lane % kLines, k0 = lane / kLines * 32;
-  const int64_t n = n0 + r < out_f ? n0 + r : out_f - 1;  // rows past the end: not stored
-  const uint8_t* wrow = w + n * in_f + k0;
-  const uint8_t* scale = ws + n0 / kBlock * blocks_k;
+  const int64_t n = n0 + r < a.out_f ? n0 + r : a.out_f - 1;  // rows past the end: not stored
+  const uint8_t* wrow = a.w + n * a.in_f + k0;
+  const uint8_t* scale = a.ws + n0 / kBlock * a.blocks_k;
   f32x4 acc[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto fetch = [&](int step, i32x8& q, int& sq) {
+  Octet<DT> x[kPieces];
+  const int per_row = (int)a.ldx / kPatch;
+  if (ENCODE) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int i = threadIdx.x + j * kLanes;
+      const int token = i / per_row, c = i % per_row * kPatch;
+      x[j] = Octet<DT>{};
+      if (token >= a.tokens) continue;
+      const int64_t at = token * a.x.stride + c;
+      if (a.vec) {
+        if (c < a.in_f) x[j].load(a.x.base, at);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPatch; ++e)
+          if (c + e < a.in_f) x[j].put(e, a.x.base, at + e);
+      }
+    }
+  }
+  auto fetch = [&](int step, i32x8& q, int& sq, i32x8 (&p)[TILES], int (&sp)[TILES]) {
     const int k = step * kStepBytes + k0;
     i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
     sq = 0;
-    if (step < blocks_k) {
-      if (k < in_f) lo = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes);
-      if (k + 16 < in_f) hi = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes + 16);
+    if (step < a.blocks_k) {
+      if (k < a.in_f) lo = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes);
+      if (k + 16 < a.in_f) hi = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes + 16);
       sq = scale[step];
     }
     q = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  i32x8 q[kFewAhead];
-  int sq[kFewAhead];
+    if constexpr (!ENCODE) {
 #pragma unroll
-  for (int i = 0; i < kFewAhead; ++i) fetch(wave + i * kFewWaves, q[i], sq[i]);
-  for (int step = wave; step < blocks_k; step += kFewAhead * kFewWaves) {
-#pragma unroll
-    for (int i = 0; i < kFewAhead; ++i) {
-      const int at = step + i * kFewWaves;
-      if (at < blocks_k) {
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          const int token = t * kLines + r;
-          i32x8 p = {0, 0, 0, 0, 0, 0, 0, 0};
-          if (token < tokens) {  // rows of codes are whole steps long
-            const uint8_t* x = xq + token * ldx + at * kStepBytes + k0;
-            p = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(x),
-                                        *reinterpret_cast<const i32x4*>(x + 16), 0, 1, 2, 3, 4, 5,
-                                        6, 7);
-          }
-          const int sp = token < tokens ? xs[packed_scale_at(token, at, xs_stride)] : 0;
-          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[i], p, acc[t], 0, 0, 0,
-                                                                    sq[i], 0, sp);
+      for (int t = 0; t < TILES; ++t) {
+        const int token = t * kLines + r;
+        p[t] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+        sp[t] = 0;
+        if (step < a.blocks_k && token < a.tokens) {  // rows of codes are whole steps long
+          const uint8_t* at = a.xq + token * a.ldx + k;
+          p[t] = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(at),
+                                         *reinterpret_cast<const i32x4*>(at + 16), 0, 1, 2, 3, 4,
+                                         5, 6, 7);
+          sp[t] = a.xs[packed_scale_at(token, step, a.xs_stride)];
         }
       }
-      fetch(at + kFewAhead * kFewWaves, q[i], sq[i]);
+    }
+  };
+  i32x8 q[kFewAhead], p[kFewAhead][TILES];
+  int sq[kFewAhead], sp[kFewAhead][TILES];
+#pragma unroll
+  for (int i = 0; i < kFewAhead; ++i) fetch(wave + i * WAVES, q[i], sq[i], p[i], sp[i]);
+
+  if (ENCODE) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int i = threadIdx.x + j * kLanes;
+      if (j * kLanes >= a.tokens * per_row) break;
+      float v[kPatch], top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPatch; ++e) {
+        v[e] = fabsf(x[j][e]) == INFINITY ? NAN : x[j][e];
+        top = fmaxf(top, fabsf(v[e]));
+      }
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      const uint32_t s = scale_of(top);
+      const float d = down_of(s);
+      *reinterpret_cast<u32x2*>(codes + i * kPatch) =
+          u32x2{encode4(v[0] * d, v[1] * d, v[2] * d, v[3] * d),
+                encode4(v[4] * d, v[5] * d, v[6] * d, v[7] * d)};
+      if (i % 16 == 0) scales[i / 16] = (uint8_t)s;
+    }
+    __syncthreads();
+  }
+  for (int step = wave; step < a.blocks_k; step += kFewAhead * WAVES) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int at = step + i * WAVES;
+      if (at < a.blocks_k) {
+        if constexpr (ENCODE) {
+          p[i][0] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+          sp[i][0] = 0;
+          if (r < a.tokens) {
+            const uint8_t* c = codes + r * (int)a.ldx + at * kStepBytes + k0;
+            p[i][0] = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(c),
+                                              *reinterpret_cast<const i32x4*>(c + 16), 0, 1, 2, 3,
+                                              4, 5, 6, 7);
+            sp[i][0] = scales[r * a.blocks_k + at];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[i], p[i][t], acc[t], 0, 0, 0,
+                                                                    sq[i], 0, sp[i][t]);
+      }
+      fetch(at + kFewAhead * WAVES, q[i], sq[i], p[i], sp[i]);
     }
   }
 #pragma unroll
@@ -482,15 +579,26 @@ fp8_few_kernel(const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, in
     *reinterpret_cast<f32x4*>(&sums[wave][t][r][lane / kLines * 4]) = acc[t];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < TILES * kLines * kLines; i += kFewWaves * kWave) {
+  for (int i = threadIdx.x; i < TILES * kLines * kLines; i += kLanes) {
     const int token = i / kLines, c = i % kLines;
-    if (token >= tokens || n0 + c >= out_f) continue;
+    if (token >= a.tokens || n0 + c >= a.out_f) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int g = 0; g < kFewWaves; ++g) v += sums[g][token / kLines][token % kLines][c];
-    if (bias) v += load1<DT>(bias, n0 + c);
-    store1<DT>(y, token * out_f + n0 + c, v);
+    for (int g = 0; g < WAVES; ++g) v += sums[g][token / kLines][token % kLines][c];
+    if (a.bias) v += load1<DT>(a.bias, n0 + c);
+    store1<DT>(a.y, token * a.out_f + n0 + c, v);
   }
+}
+
+template <int DT, int TILES, bool ENCODE>
+void launch_few(const Few<DT>& a, int waves, hipStream_t s) {
+  const dim3 grid((unsigned)tiles_along(a.out_f, kLines)), block(waves * kWave);
+  if (waves == 4)
+    hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 4, ENCODE>), grid, block, 0, s, a);
+  else if (waves == 8)
+    hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 8, ENCODE>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 16, ENCODE>), grid, block, 0, s, a);
 }
 
 template <int DT>
@@ -500,6 +608,7 @@ fp8_join_kernel(const float* __restrict__ part, int slices, int64_t count, int64
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (i >= count) return;
   float v = part[i];
+#pragma unroll 8
   for (int s = 1; s < slices; ++s) v += part[s * count + i];
   if (bias) v += load1<DT>(bias, i % cols);
   store1<DT>(out, i, v);
@@ -533,11 +642,6 @@ int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hi
   return launch_status();
 }
 
-struct Source {
-  const void* base;
-  int64_t stride, rows, cols;
-};
-
 bool vector_rows(const Source& m, int dtype) {
   const int64_t per = dtype == OA_F32 ? 4 : 8;
   return m.cols % 8 == 0 && m.stride % per == 0 && aligned_to(m.base, 16);
@@ -559,56 +663,63 @@ int encode_rows(const Source& m, const Encoded& e, hipStream_t s) {
   return launch_status();
 }
 
-// Up to this many tokens the weight's bytes are what the product takes; a tile of 128
-// tokens in slices took 14 + 4 us where 58 MB can be read in 11.
-constexpr int64_t kFewTokens = 64;
-
 struct Layer {
   const uint8_t *q, *scales;
   int64_t out_f, in_f;
 };
 
+// Whether the kernel for few tokens takes a call.  It reads every token's codes once per 16
+// columns, the tiles once per 128, but those take two more launches and half the bytes they
+// move in LDS are for rows that hold no token.  4096 -> 14336: 15, 17 and 24 us for 1, 4 and
+// 16 tokens, 22 with tiles; 28 against 22 for 24; a small weight gains for longer: 4096 ->
+// 4096, 24 tokens, 11 against 15, 64 tokens 16 and 16.
+bool takes_few(const Layer& w, int64_t tokens) {
+  return tokens <= kLines || (tokens <= 2 * kLines && w.out_f * w.in_f <= (1 << 24));
+}
+// Waves of its workgroups: a CU that has only one of them needs more loads in flight from
+// it.  1 token, 4 / 8 / 16 waves: 4096 -> 14336, 15.4, 16.1, 19.5 us; 14336 -> 4096, 22.3,
+// 15.8, 13.5; 4096 -> 4096, 8.0, 6.4, 6.3; 2048 -> 5632, 5.6, 6.0, 7.6.
+int few_waves(const Layer& w) {
+  if (tiles_along(w.out_f, kLines) > 256) return 4;
+  return blocks_of(w.in_f) < 64 ? 8 : 16;
+}
+
 struct ForwardPlan {
   Encoded x{};
   Output y;
   size_t bytes;
-  ForwardPlan(int64_t tokens, int64_t in_f, int64_t out_f, void* ws) {
+  ForwardPlan(int64_t tokens, int64_t in_f, int64_t out_f, bool few, void* ws) {
     Carver c{static_cast<uint8_t*>(ws)};
     x.ld = up_to(in_f, kBlock);
     x.scale_stride = up_to(tokens, 256);
     x.q = c.take<uint8_t>(tokens * x.ld);
     x.scales = c.take<uint8_t>(blocks_of(in_f) * x.scale_stride);
-    if (tokens > kFewTokens) y = Output(tokens, out_f, in_f, c);
+    if (!few) y = Output(tokens, out_f, in_f, c);
     bytes = c.used;
   }
 };
 
 template <int DT>
 int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws, hipStream_t s) {
-  const ForwardPlan plan(x.rows, w.in_f, w.out_f, ws);
-  int rc = encode_rows<DT>(x, plan.x, s);
-  if (rc) return rc;
-  if (x.rows <= kFewTokens) {
-    const dim3 grid((unsigned)tiles_along(w.out_f, kLines)), block(kFewWaves * kWave);
-    const int blocks = (int)blocks_of(w.in_f), tokens = (int)x.rows;
-    switch (tiles_along(x.rows, kLines)) {
-      case 1:
-        hipLaunchKernelGGL((fp8_few_kernel<DT, 1>), grid, block, 0, s, w.q, w.scales, w.out_f,
-                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
-                           plan.x.scale_stride, tokens, bias, y);
-        break;
-      case 2:
-        hipLaunchKernelGGL((fp8_few_kernel<DT, 2>), grid, block, 0, s, w.q, w.scales, w.out_f,
-                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
-                           plan.x.scale_stride, tokens, bias, y);
-        break;
-      default:
-        hipLaunchKernelGGL((fp8_few_kernel<DT, 4>), grid, block, 0, s, w.q, w.scales, w.out_f,
-                           (int)w.in_f, blocks, plan.x.q, plan.x.scales, plan.x.ld,
-                           plan.x.scale_stride, tokens, bias, y);
+  const bool few = takes_few(w, x.rows);
+  const ForwardPlan plan(x.rows, w.in_f, w.out_f, few, ws);
+  if (few) {
+    const int waves = few_waves(w), tokens = (int)x.rows;
+    const Few<DT> a{w.q, w.scales, w.out_f, (int)w.in_f, (int)blocks_of(w.in_f),
+                    x, vector_rows(x, DT), plan.x.q, plan.x.scales, plan.x.ld,
+                    plan.x.scale_stride, tokens, bias, y};
+    if (tokens <= kFewEncodeTokens && tokens * plan.x.ld <= kFewCodes) {
+      launch_few<DT, 1, true>(a, waves, s);
+      return launch_status();
     }
+    const int rc = encode_rows<DT>(x, plan.x, s);
+    if (rc) return rc;
+    if (tokens <= kLines) launch_few<DT, 1, false>(a, waves, s);
+    else launch_few<DT, 2, false>(a, waves, s);
     return launch_status();
   }
+  int rc = encode_rows<DT>(x, plan.x, s);
+  if (rc) return rc;
   Problem pr{};
   pr.q = Operand{w.q, w.in_f, w.out_f, 0};
   pr.p = Operand{plan.x.q, plan.x.ld, x.rows, 0};
@@ -784,7 +895,10 @@ extern "C" size_t oa_fp8_linear_workspace_bytes(int64_t tokens, int64_t in_featu
                                                 int64_t out_features, int backward, int want_dx,
                                                 int want_dw, int want_db) {
   if (tokens <= 0 || in_features <= 0 || out_features <= 0) return 0;
-  if (!backward) return ForwardPlan(tokens, in_features, out_features, nullptr).bytes;
+  if (!backward) {
+    const bool few = takes_few(Layer{nullptr, nullptr, out_features, in_features}, tokens);
+    return ForwardPlan(tokens, in_features, out_features, few, nullptr).bytes;
+  }
   return BackwardPlan(tokens, in_features, out_features, want_dx != 0, want_dw != 0, want_db != 0,
                       nullptr)
       .bytes;

@@ -29,7 +29,7 @@ namespace {
 using namespace gemm;
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kCombineTokens = 32, kCombineParts = 8;
+constexpr int kCombineTokens = 8, kCombineParts = 32;
 constexpr int kCombineThreads = kCombineTokens * kCombineParts;
 constexpr int kReduceThreads = 1024;
 
@@ -121,30 +121,39 @@ struct StatsEpilogue {
   }
 };
 
-// Joins a token's tiles: eight lanes per token, then the eight.  A target outside
-// [0, vocab) that is not `ignore` makes the loss NaN.
+// Joins a token's tiles: 32 lanes per token, eight to a wave, then the lanes (a chain of
+// loads and exponentials is what this takes: 8 us with 8 lanes per token and 125 tiles, 4
+// with 32).  A target outside [0, vocab) that is not `ignore` makes the loss NaN.
 __global__ void __launch_bounds__(kCombineThreads)
 ce_combine_kernel(const f32x2* __restrict__ part, const float* __restrict__ z_target,
                   const int64_t* __restrict__ target, int64_t tokens, int64_t vocab,
                   int64_t ignore, int tiles, float* __restrict__ lse_out,
                   float* __restrict__ loss_out, float* __restrict__ block_sum,
                   int* __restrict__ block_count) {
-  __shared__ f32x2 all[kCombineParts][kCombineTokens];
+  __shared__ f32x2 all[kCombineThreads / kWave][kCombineTokens];
   const int col = threadIdx.x % kCombineTokens, row = threadIdx.x / kCombineTokens;
   const int64_t token = (int64_t)blockIdx.x * kCombineTokens + col;
   float m = -INFINITY, s = 0.0f;
-  if (token < tokens)
+  if (token < tokens) {
+#pragma unroll 4
     for (int j = row; j < tiles; j += kCombineParts) {
       const f32x2 v = part[(int64_t)j * tokens + token];
       join(m, s, v[0], v[1]);
     }
-  all[row][col] = f32x2{m, s};
+  }
+#pragma unroll
+  for (int off = kCombineTokens; off < kWave; off <<= 1) {
+    const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
+    join(m, s, m2, s2);
+  }
+  if (threadIdx.x % kWave < kCombineTokens) all[threadIdx.x / kWave][col] = f32x2{m, s};
   __syncthreads();
   if (threadIdx.x >= kWave) return;
   float loss = 0.0f;
   bool used = false;
   if (threadIdx.x < kCombineTokens && token < tokens) {
-    for (int j = 1; j < kCombineParts; ++j) join(m, s, all[j][col][0], all[j][col][1]);
+#pragma unroll
+    for (int w = 1; w < kCombineThreads / kWave; ++w) join(m, s, all[w][col][0], all[w][col][1]);
     const float lse = m + logf(s);
     lse_out[token] = lse;
     const int64_t y = target[token];
@@ -186,7 +195,7 @@ ce_reduce_kernel(const float* __restrict__ block_sum, const int* __restrict__ bl
     c += counts[w];
   }
   *count_out = (float)c;
-  if (loss_out) *loss_out = mean ? s / (float)c : s;  // nothing took part: 0 / 0
+  *loss_out = mean ? s / (float)c : s;  // nothing took part: 0 / 0
 }
 
 // ------------------------------------------------------------------ backward
@@ -343,6 +352,7 @@ ce_dx_kernel(const float* __restrict__ sum, int slices, const float* __restrict_
   if (i >= quads) return;
   const float f = factor[i * 4 / hidden];
   f32x4 v = reinterpret_cast<const f32x4*>(sum)[i];
+#pragma unroll 8
   for (int s = 1; s < slices; ++s) v += reinterpret_cast<const f32x4*>(sum)[s * quads + i];
   v = f == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * f;
   reinterpret_cast<u32x2*>(dx)[i] =
@@ -468,9 +478,9 @@ int forward(const Head& h, int reduction, float* loss, float* lse, float* count,
     rc = launch_status();
     if (rc) return rc;
   }
+  if (reduction == OA_LOSS_NONE) return 0;
   hipLaunchKernelGGL(ce_reduce_kernel, dim3(1), dim3(kReduceThreads), 0, s, plan.block_sum,
-                     plan.block_count, plan.blocks, reduction == OA_LOSS_MEAN,
-                     reduction == OA_LOSS_NONE ? nullptr : loss, count);
+                     plan.block_count, plan.blocks, reduction == OA_LOSS_MEAN, loss, count);
   return launch_status();
 }
 

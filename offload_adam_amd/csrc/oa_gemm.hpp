@@ -773,27 +773,33 @@ struct Cut {
   int slices;
 };
 
-// The cut with the least estimated time, in microseconds: rounds of workgroups times (steps
-// of a slice times the time of one, plus what a tile costs besides), and the traffic of
-// partial results.  Measured with both element types: 1.4 to 1.7 a step and 7 besides for
-// the large tile, 1.0 and 2 for a round of small ones; partial sums move at some 4 TB/s.
-// e4m3, 4096 x 5632 x 2048: 52 us small (54 estimated), 62 estimated large; 4096 x 2048 x
-// 5632: 46 + 16 large in two slices, 46 estimated small; 4096 x 14336 x 4096: 211 large,
-// 270 small; bf16, 4096 x 2048 x 16384: 190 large in two slices, 260 small.
+// The cut with the least estimated time, in microseconds.  A round of n workgroups takes
+// steps times the time of a step, plus what a tile costs besides.  The time of a step grows
+// with n, as the loads of more CUs meet and the clock falls: from 0.95 to 1.5 for the large
+// tile, from 0.42 to 0.95 for the small one, measured with both element types.  Slices add
+// a launch, the traffic of partial sums (some 4 TB/s) and a chain of loads.
+// e4m3, 4096 x 5632 x 2048: 52 us small, 58 large; 4096 x 14336 x 4096: 209 large, 248
+// small; bf16, 4096 x 2048 x 16384: 190 large in two slices, 260 small; 484 x 232 x 37632:
+// 29 small in 12 slices, 40 in 49.
 inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, bool may_slice) {
   Cut best{false, 1};
   double least = 0.0;
   for (int large = 0; large < 2; ++large) {
     const int64_t side = large ? 256 : 128, room = large ? 256 : 512;
-    const double step = large ? 1.5 : 1.0, besides = large ? 7.0 : 2.0;
+    const double base = large ? 0.95 : 0.42, more = large ? 0.55 : 0.53;
+    const double besides = large ? 7.0 : 3.0;
     const int64_t tiles = tiles_along(rows_q, side) * tiles_along(rows_p, side);
     int64_t most = may_slice ? room / tiles : 1;  // a full chip is not cut further
     if (most > steps / 4) most = steps / 4;
     if (most < 1) most = 1;
     for (int64_t slices = 1; slices <= most; ++slices) {
-      double t = (double)tiles_along(tiles * slices, room) *
-                 ((double)tiles_along(steps, slices) * step + besides);
-      if (slices > 1) t += 5.0 + (double)rows_q * (double)rows_p * 8.0 * (double)slices / 4e6;
+      const int64_t n = tiles * slices, rest = n % room;
+      const double s = (double)tiles_along(steps, slices);
+      double t = (double)(n / room) * (s * (base + more) + besides);
+      if (rest) t += s * (base + more * (double)rest / (double)room) + besides;
+      if (slices > 1)
+        t += 3.0 + 0.1 * (double)slices +
+             (double)rows_q * (double)rows_p * 8.0 * (double)slices / 4e6;
       if (least == 0.0 || t < least) {
         least = t;
         best = Cut{large != 0, (int)slices};
