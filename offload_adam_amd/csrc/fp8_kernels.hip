@@ -14,6 +14,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "oa_gemm.hpp"
 
 #pragma clang fp contract(off)
@@ -111,27 +113,68 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// One lane's 8 x 8 patch of a source: rows r0 .. r0+7, columns c0 .. c0+7; what lies
-// outside reads as zero, infinities as NaN.  `vec`: rows are 16-byte aligned and a
-// multiple of 8 columns long.
+// A matrix to encode: rows `stride` elements apart.
+struct Source {
+  const void* base;
+  int64_t stride, rows, cols;
+};
+
+// Largest of 16 neighbouring lanes, in all of them.
+__device__ __forceinline__ float max_of_16(float v) {
+  auto other = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xF,
+                                                   0xF, true));
+  };
+  v = fmaxf(v, other(v, std::integral_constant<int, 0xB1>{}));   // 1 0 3 2 of each four
+  v = fmaxf(v, other(v, std::integral_constant<int, 0x4E>{}));   // 2 3 0 1
+  v = fmaxf(v, other(v, std::integral_constant<int, 0x141>{}));  // mirrored eights
+  return fmaxf(v, other(v, std::integral_constant<int, 0x140>{}));  // mirrored sixteens
+}
+
+// One lane's 8 x 8 patch of block (br, bc): rows r .. r+7, columns c .. c+7 of it; what lies
+// outside the source reads as zero.  `vec`: rows are 16-byte aligned, whole octets, and
+// 128 of them span less than 2^31 bytes.
 template <int DT>
-__device__ __forceinline__ void load_patch(const void* src, int64_t stride, int64_t rows,
-                                           int64_t cols, int64_t r0, int64_t c0, bool vec,
-                                           float (&v)[kPatch][kPatch]) {
-  float top = 0.0f;
+__device__ __forceinline__ void load_patch(const Source& m, int64_t br, int64_t bc, int r, int c,
+                                           bool vec, float (&v)[kPatch][kPatch]) {
+  constexpr int kSize = DT == OA_F32 ? 4 : 2;
+  const int64_t first = br * kBlock, left = m.rows - first, c0 = bc * kBlock + c;
+  const int rows = left < kBlock ? (int)left : kBlock;
+  if (vec) {
+    const uint8_t* base = static_cast<const uint8_t*>(m.base) + first * m.stride * kSize;
+    const int pitch = (int)m.stride * kSize;
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base), 0, (rows - 1) * pitch + (int)m.cols * kSize, 0x00020000);
+    const int at = c0 < m.cols ? r * pitch + (int)c0 * kSize : kOut;
+    Octet<DT> o[kPatch];
 #pragma unroll
-  for (int p = 0; p < kPatch; ++p) {
+    for (int p = 0; p < kPatch; ++p)
 #pragma unroll
-    for (int j = 0; j < kPatch; ++j) v[p][j] = 0.0f;
-    if (r0 + p >= rows) continue;
-    if (vec) {
-      if (c0 < cols) load8<DT>(src, (r0 + p) * stride + c0, v[p]);
-    } else {
+      for (int k = 0; k < Octet<DT>::kWords; ++k)
+        o[p].w[k] = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       rsrc, r + p < rows ? at + p * pitch + 16 * k : kOut, 0, 0));
 #pragma unroll
-      for (int j = 0; j < kPatch; ++j)
-        if (c0 + j < cols) v[p][j] = load1<DT>(src, (r0 + p) * stride + c0 + j);
+    for (int p = 0; p < kPatch; ++p)
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j) v[p][j] = o[p][j];
+  } else {
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p) {
+      const int64_t row = (first + (r + p < rows ? r + p : 0)) * m.stride;
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j) {
+        const bool in = r + p < rows && c0 + j < m.cols;
+        const float x = load1<DT>(m.base, row + (c0 + j < m.cols ? c0 + j : 0));
+        v[p][j] = in ? x : 0.0f;
+      }
     }
   }
+}
+
+// Infinities of a patch as NaN: they have no code.
+__device__ __forceinline__ void drop_infinities(float (&v)[kPatch][kPatch]) {
+  float top = 0.0f;
 #pragma unroll
   for (int p = 0; p < kPatch; ++p)
 #pragma unroll
@@ -150,15 +193,15 @@ __device__ __forceinline__ void load_patch(const void* src, int64_t stride, int6
 // One workgroup per 128 x 128 block: one read of the source, one write of the codes.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_encode_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
-                  int64_t blocks_c, bool vec, uint8_t* __restrict__ q,
+fp8_encode_kernel(const Source m, uint32_t blocks_c, bool vec, uint8_t* __restrict__ q,
                   uint8_t* __restrict__ scales) {
   __shared__ float tops[kThreads / kWave];
   const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
-  const int64_t r0 = br * kBlock + threadIdx.x / 16 * kPatch;
-  const int64_t c0 = bc * kBlock + threadIdx.x % 16 * kPatch;
+  const int r = threadIdx.x / 16 * kPatch, c = threadIdx.x % 16 * kPatch;
+  const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
   float v[kPatch][kPatch];
-  load_patch<DT>(src, stride, rows, cols, r0, c0, vec, v);
+  load_patch<DT>(m, br, bc, r, c, vec, v);
+  drop_infinities(v);
   float top = 0.0f;
 #pragma unroll
   for (int p = 0; p < kPatch; ++p)
@@ -174,9 +217,9 @@ fp8_encode_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, in
   if (threadIdx.x == 0) scales[blockIdx.x] = (uint8_t)s;
 #pragma unroll
   for (int p = 0; p < kPatch; ++p) {
-    if (r0 + p >= rows || c0 >= cols) continue;  // cols is a multiple of 16
+    if (r0 + p >= m.rows || c0 >= m.cols) continue;  // a multiple of 16 columns
     float* x = v[p];
-    *reinterpret_cast<u32x2*>(q + (r0 + p) * cols + c0) =
+    *reinterpret_cast<u32x2*>(q + (r0 + p) * m.cols + c0) =
         u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
               encode4(x[4] * down, x[5] * down, x[6] * down, x[7] * down)};
   }
@@ -229,31 +272,75 @@ struct Encoded {
   float* sums;       // [row block][cols]: sums over 128 rows
 };
 
+// One workgroup per 128 x 128 block.  4096 x 14336 in bf16 to both kinds of codes: 52
+// us for 235 MB.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_operand_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
-                   int64_t blocks_c, bool vec, const Encoded e) {
-  __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];  // [column][row]
-  __shared__ float part[16][kBlock + 4];
-  __shared__ uint32_t shared_scale[kBlock];
+fp8_operand_kernel(const Source m, uint32_t blocks_c, bool vec, const Encoded e) {
+  constexpr int kWaves = kThreads / kWave;
+  // [column][row], 16-byte pieces of a column at piece ^ (column / 16): lanes that write
+  // together meet different banks
+  __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];
+  __shared__ __align__(16) float part[kWaves][kBlock];
   const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
-  const int rg = threadIdx.x / 16, cg = threadIdx.x % 16;
+  const int wave = threadIdx.x / kWave, rg = threadIdx.x / 16, cg = threadIdx.x % 16;
   const int r = rg * kPatch, c = cg * kPatch;
   const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
   float v[kPatch][kPatch];
-  load_patch<DT>(src, stride, rows, cols, r0, c0, vec, v);
+  load_patch<DT>(m, br, bc, r, c, vec, v);
 
+  // one number per column of this lane's, from its rows, over the rows of the block
+  auto over_rows = [&](float (&a)[kPatch], auto join) {
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) {
+      a[j] = join(a[j], __shfl_xor(a[j], 16, kWave));
+      a[j] = join(a[j], __shfl_xor(a[j], 32, kWave));
+    }
+    if (threadIdx.x % kWave < 16) {
+#pragma unroll
+      for (int j = 0; j < kPatch; j += 4)
+        *reinterpret_cast<f32x4*>(&part[wave][c + j]) = f32x4{a[j], a[j + 1], a[j + 2], a[j + 3]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPatch; j += 4) {
+      f32x4 all = *reinterpret_cast<const f32x4*>(&part[0][c + j]);
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const f32x4 one = *reinterpret_cast<const f32x4*>(&part[w][c + j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all[i] = join(all[i], one[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[j + i] = all[i];
+    }
+  };
+  if (e.sums) {
+    float s[kPatch];
+#pragma unroll
+    for (int j = 0; j < kPatch; ++j) {
+      s[j] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kPatch; ++p) s[j] += v[p][j];
+    }
+    over_rows(s, [](float a, float b) { return a + b; });
+    if (rg == 0) {
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j)
+        if (c0 + j < m.cols) e.sums[br * m.cols + c0 + j] = s[j];
+    }
+    __syncthreads();
+  }
+  drop_infinities(v);
   if (e.q) {
 #pragma unroll
     for (int p = 0; p < kPatch; ++p) {
       float top = 0.0f;
 #pragma unroll
       for (int j = 0; j < kPatch; ++j) top = fmaxf(top, fabsf(v[p][j]));
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-      const uint32_t s = scale_of(top);
+      const uint32_t s = scale_of(max_of_16(top));
       const float down = down_of(s);
-      if (r0 + p < rows) {
+      if (r0 + p < m.rows) {
         const float* x = v[p];
         *reinterpret_cast<u32x2*>(e.q + (r0 + p) * e.ld + c0) =
             u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
@@ -262,54 +349,32 @@ fp8_operand_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, i
       }
     }
   }
-  if (e.sums) {
-#pragma unroll
-    for (int j = 0; j < kPatch; ++j) {
-      float s = 0.0f;
-#pragma unroll
-      for (int p = 0; p < kPatch; ++p) s += v[p][j];
-      part[rg][c + j] = s;
-    }
-    __syncthreads();
-    if (threadIdx.x < kBlock && bc * kBlock + threadIdx.x < cols) {
-      float s = 0.0f;
-      for (int g = 0; g < 16; ++g) s += part[g][threadIdx.x];
-      e.sums[br * cols + bc * kBlock + threadIdx.x] = s;
-    }
-    __syncthreads();
-  }
   if (!e.qt) return;
+  float top[kPatch];
 #pragma unroll
   for (int j = 0; j < kPatch; ++j) {
-    float top = 0.0f;
+    top[j] = 0.0f;
 #pragma unroll
-    for (int p = 0; p < kPatch; ++p) top = fmaxf(top, fabsf(v[p][j]));
-    part[rg][c + j] = top;
+    for (int p = 0; p < kPatch; ++p) top[j] = fmaxf(top[j], fabsf(v[p][j]));
   }
-  __syncthreads();
-  if (threadIdx.x < kBlock) {
-    float top = 0.0f;
-    for (int g = 0; g < 16; ++g) top = fmaxf(top, part[g][threadIdx.x]);
-    const uint32_t s = scale_of(top);
-    shared_scale[threadIdx.x] = s;
-    const int64_t col = bc * kBlock + threadIdx.x;
-    if (col < cols) e.scales_t[packed_scale_at(col, br, e.scale_stride_t)] = (uint8_t)s;
-  }
-  __syncthreads();
+  over_rows(top, [](float a, float b) { return fmaxf(a, b); });
 #pragma unroll
   for (int j = 0; j < kPatch; ++j) {
-    const float d = down_of(shared_scale[c + j]);
-    *reinterpret_cast<u32x2*>(&tile[c + j][r]) =
+    const uint32_t s = scale_of(top[j]);
+    const float d = down_of(s);
+    if (rg == 0 && c0 + j < m.cols)
+      e.scales_t[packed_scale_at(c0 + j, br, e.scale_stride_t)] = (uint8_t)s;
+    *reinterpret_cast<u32x2*>(&tile[c + j][(rg / 2 ^ cg / 2) * 16 + rg % 2 * 8]) =
         u32x2{encode4(v[0][j] * d, v[1][j] * d, v[2][j] * d, v[3][j] * d),
               encode4(v[4][j] * d, v[5][j] * d, v[6][j] * d, v[7][j] * d)};
   }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int i = threadIdx.x + kThreads * k, col = i / 8, piece = i % 8 * 16;
-    if (bc * kBlock + col < cols)
-      *reinterpret_cast<u32x4*>(e.qt + (bc * kBlock + col) * e.ld_t + br * kBlock + piece) =
-          *reinterpret_cast<const u32x4*>(&tile[col][piece]);
+    const int i = threadIdx.x + kThreads * k, col = i / 8, piece = i % 8;
+    if (bc * kBlock + col < m.cols)
+      *reinterpret_cast<u32x4*>(e.qt + (bc * kBlock + col) * e.ld_t + br * kBlock + piece * 16) =
+          *reinterpret_cast<const u32x4*>(&tile[col][(piece ^ col / 16) * 16]);
   }
 }
 
@@ -317,19 +382,18 @@ fp8_operand_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, i
 // block, eight elements to a lane, columns from `cols` up to e.ld zero.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_rows_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int64_t cols, bool vec,
-                const Encoded e) {
+fp8_rows_kernel(const Source m, bool vec, const Encoded e) {
   const int64_t per_row = e.ld / kPatch;
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t r = i / per_row, c = i % per_row * kPatch;
-  if (r >= rows) return;  // 16 lanes together: rows are whole blocks long
+  if (r >= m.rows) return;  // 16 lanes together: rows are whole blocks long
   float x[kPatch] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   if (vec) {
-    if (c < cols) load8<DT>(src, r * stride + c, x);
+    if (c < m.cols) load8<DT>(m.base, r * m.stride + c, x);
   } else {
 #pragma unroll
     for (int j = 0; j < kPatch; ++j)
-      if (c + j < cols) x[j] = load1<DT>(src, r * stride + c + j);
+      if (c + j < m.cols) x[j] = load1<DT>(m.base, r * m.stride + c + j);
   }
   float top = 0.0f;
 #pragma unroll
@@ -337,9 +401,7 @@ fp8_rows_kernel(const void* __restrict__ src, int64_t stride, int64_t rows, int6
     if (fabsf(x[j]) == INFINITY) x[j] = NAN;
     top = fmaxf(top, fabsf(x[j]));
   }
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-  const uint32_t s = scale_of(top);
+  const uint32_t s = scale_of(max_of_16(top));
   const float down = down_of(s);
   *reinterpret_cast<u32x2*>(e.q + r * e.ld + c) =
       u32x2{encode4(x[0] * down, x[1] * down, x[2] * down, x[3] * down),
@@ -425,11 +487,6 @@ struct SliceEpilogue {
     const StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr, vec};
     e(t, row_q, row_p, tq, 0, lds);
   }
-};
-
-struct Source {
-  const void* base;
-  int64_t stride, rows, cols;
 };
 
 // ---- few tokens.  Bound by reading the weight once.  A workgroup makes 16 columns of y;
@@ -538,9 +595,7 @@ __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) 
         v[e] = fabsf(x[j][e]) == INFINITY ? NAN : x[j][e];
         top = fmaxf(top, fabsf(v[e]));
       }
-#pragma unroll
-      for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-      const uint32_t s = scale_of(top);
+      const uint32_t s = scale_of(max_of_16(top));
       const float d = down_of(s);
       *reinterpret_cast<u32x2*>(codes + i * kPatch) =
           u32x2{encode4(v[0] * d, v[1] * d, v[2] * d, v[3] * d),
@@ -644,14 +699,15 @@ int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hi
 
 bool vector_rows(const Source& m, int dtype) {
   const int64_t per = dtype == OA_F32 ? 4 : 8;
-  return m.cols % 8 == 0 && m.stride % per == 0 && aligned_to(m.base, 16);
+  return m.cols % 8 == 0 && m.stride % per == 0 && m.stride < (1 << 21) && m.cols < (1 << 21) &&
+         aligned_to(m.base, 16);
 }
 
 template <int DT>
 int encode_operand(const Source& m, const Encoded& e, hipStream_t s) {
   const int64_t bc = blocks_of(m.cols), br = blocks_of(m.rows);
-  hipLaunchKernelGGL(fp8_operand_kernel<DT>, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s,
-                     m.base, m.stride, m.rows, m.cols, bc, vector_rows(m, DT), e);
+  hipLaunchKernelGGL(fp8_operand_kernel<DT>, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s, m,
+                     (uint32_t)bc, vector_rows(m, DT), e);
   return launch_status();
 }
 
@@ -659,7 +715,7 @@ template <int DT>
 int encode_rows(const Source& m, const Encoded& e, hipStream_t s) {
   const int64_t lanes = m.rows * (e.ld / kPatch);
   hipLaunchKernelGGL(fp8_rows_kernel<DT>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, s, m.base, m.stride, m.rows, m.cols, vector_rows(m, DT), e);
+                     dim3(kThreads), 0, s, m, vector_rows(m, DT), e);
   return launch_status();
 }
 
@@ -842,22 +898,19 @@ extern "C" int oa_quant_fp8(const void* src, int src_dtype, int64_t src_row_stri
   rc = check_source(m, src_dtype);
   if (rc) return rc;
   const bool vec = vector_rows(m, src_dtype);
-  const int64_t bc = blocks_of(cols);
+  const uint32_t bc = (uint32_t)blocks_of(cols);
   const dim3 grid((unsigned)(bc * blocks_of(rows)));
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t *qb = static_cast<uint8_t*>(q), *sb = static_cast<uint8_t*>(scales);
   switch (src_dtype) {
     case OA_F32:
-      hipLaunchKernelGGL(fp8_encode_kernel<OA_F32>, grid, dim3(kThreads), 0, s, src,
-                         src_row_stride, rows, cols, bc, vec, qb, sb);
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_F32>, grid, dim3(kThreads), 0, s, m, bc, vec, qb, sb);
       break;
     case OA_BF16:
-      hipLaunchKernelGGL(fp8_encode_kernel<OA_BF16>, grid, dim3(kThreads), 0, s, src,
-                         src_row_stride, rows, cols, bc, vec, qb, sb);
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_BF16>, grid, dim3(kThreads), 0, s, m, bc, vec, qb, sb);
       break;
     default:
-      hipLaunchKernelGGL(fp8_encode_kernel<OA_F16>, grid, dim3(kThreads), 0, s, src,
-                         src_row_stride, rows, cols, bc, vec, qb, sb);
+      hipLaunchKernelGGL(fp8_encode_kernel<OA_F16>, grid, dim3(kThreads), 0, s, m, bc, vec, qb, sb);
   }
   return launch_status();
 }

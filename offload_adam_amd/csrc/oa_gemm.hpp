@@ -173,6 +173,8 @@ __device__ __forceinline__ i32x4 descriptor(const uint8_t* base, int bytes) {
   return r;
 }
 
+constexpr int kOut = 0x60000000;  // out of any descriptor's range
+
 // Descriptor of a tile's rows from byte k of the first on: what is not in the range reads
 // as zero, among it every row past the operand's last.
 __device__ __forceinline__ i32x4 tile_rsrc(const Operand& o, int64_t row0, int tile_rows,
@@ -222,7 +224,6 @@ struct Tile {
   static constexpr int kEarly = kUnits - 8;                // units loaded in a step's first half
   static constexpr int kScaleBytes = T::kScaled ? 512 : 0; // of a step: 64 dwords of q, 64 of p
   static constexpr int kLdsBytes = kUnits * kUnitBytes + 3 * kScaleBytes;
-  static constexpr int kOut = 0x60000000;  // out of any descriptor's range
   static_assert(R == 128 || R == 64, "scales come in groups of 128 rows");
 
   // A lane's results: kQuads groups of four consecutive q for each of kColumns p; quad u

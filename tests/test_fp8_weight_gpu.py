@@ -167,6 +167,39 @@ def test_linear_and_its_gradients(shape, dtype):
            codes=False)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", [(1, 14336, 70), (1, 144, 4200), (4, 4096, 4117), (7, 2064, 33),
+                                   (16, 1024, 300), (16, 1040, 50), (12, 8400, 50), (17, 8400, 70),
+                                   (32, 400, 4200), (32, 2064, 19), (33, 2064, 19), (64, 48, 70)])
+def test_few_tokens(shape, dtype):
+    """Both sides of what decides how few tokens are multiplied: how many, where their codes
+    are made, how many waves share a column, whether rows can be read in octets."""
+    t, k, n = shape
+    x, q, b, _ = _layer(t, k, n, dtype, seed=sum(shape), bias=True)
+    x, w = x.detach(), q.detach().dequantize(F32).double()
+    y = F.linear(x, q.detach(), b.detach())
+    _close(y, _held(x, 1), w.t(), "y", b.detach().double())
+    wide = torch.zeros(t, k + 11, dtype=dtype, device="cuda")
+    wide[:, 3:3 + k] = x
+    assert torch.equal(F.linear(wide[:, 3:3 + k], q.detach(), b.detach()), y)
+    if t > 1:
+        x[0, -1], x[-1, 0] = float("nan"), float("-inf")
+        bad = F.linear(x, q.detach(), b.detach())
+        assert torch.isnan(bad[[0, -1]]).all() and torch.equal(bad[1:-1], y[1:-1])
+
+
+def test_the_bias_gradient_is_the_plain_sum():
+    """Infinities and NaN stay in their columns, and stay what they are."""
+    x, q, b, gy = _layer(300, 144, 130, BF16, bias=True)
+    gy[7, 3], gy[200, 3], gy[8, 40], gy[9, 129] = *2 * [float("inf")], float("-inf"), float("nan")
+    db, = torch.autograd.grad(F.linear(x, q, b), b, gy)
+    assert db[3] == float("inf") and db[40] == float("-inf") and torch.isnan(db[129])
+    keep = torch.ones(130, dtype=torch.bool, device="cuda")
+    keep[[3, 40, 129]] = False
+    _close(db[None, keep], torch.ones(1, 300, dtype=torch.float64, device="cuda"),
+           gy[:, keep].double(), "db", codes=False)
+
+
 @pytest.mark.parametrize("shape", [(4096, 512, 3200), (3000, 2048, 4000)])
 def test_large_tiles(shape):
     t, k, n = shape

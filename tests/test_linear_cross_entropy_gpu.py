@@ -124,6 +124,18 @@ def test_many_pieces_and_large_tiles(shape):
         _close(g, want, f"{shape} {what}")
 
 
+@pytest.mark.parametrize("shape", [(1, 64, 70001), (4, 80, 60001), (9, 8, 33000)])
+def test_few_tokens_of_a_large_vocabulary(shape):
+    """Hundreds of tiles to join per token, and dx in many slices."""
+    x, w, y = _inputs(*shape, BF16, seed=2, ignore=0.0)
+    for reduction in ("sum", "none"):
+        grad = _grad_for(reduction, shape[0])
+        got = _run(x, w, y, grad, reduction=reduction)
+        want = _expected(x, w, y, grad, reduction)
+        for g, e, what in zip(got, want, ("loss", "dx", "dw")):
+            _close(g, e, f"{shape} {reduction} {what}")
+
+
 def test_large_logits_and_confident_rows():
     """Logits of some hundreds: exponentials that vanish, probabilities of 1."""
     t, h, v = 70, 64, 700
