@@ -462,6 +462,7 @@ struct StoreEpilogue {
             const f32x4 v = t.quad(u, b);
             return u32x2{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3])};
           },
+          [] {},
           [&](int p, int q, u32x4 v) {
             if (row_p + p >= rows) return;
             uint16_t* o = static_cast<uint16_t*>(out) + (row_p + p) * cols + row_q + q;

@@ -60,6 +60,40 @@ struct Store16<F16> {
   }
 };
 
+// A token's column among a lane's (kLines * u + i for element i of quad u), or -1.  Few
+// tiles hold the target of any of their tokens, so what is done for it stays out of the
+// loops over all logits.
+template <class Tl>
+__device__ __forceinline__ int column_of(int64_t rel) {
+  return rel >= 0 && rel < Tl::kQuads * kLines && rel % kLines < 4 ? (int)rel : -1;
+}
+template <class Tl>
+__device__ __forceinline__ float logit_at(const Tl& t, int b, int rel) {
+  float z = 0.0f;
+#pragma unroll
+  for (int u = 0; u < Tl::kQuads; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (rel == kLines * u + i) z = t.quad(u, b)[i];
+  return z;
+}
+
+// A lane's columns from `left` on hold no logit: their exponentials are 0.  `any`: the tile
+// has such columns.
+template <class Tl>
+__device__ __forceinline__ void drop_columns(Tl& t, int64_t left, bool any) {
+  if (!any) return;
+#pragma unroll
+  for (int u = 0; u < Tl::kQuads; ++u)
+#pragma unroll
+    for (int b = 0; b < Tl::kColumns; ++b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (kLines * u + i >= left) t.acc[u][b][i] = -INFINITY;
+      asm volatile("" : "+a"(t.acc[u][b]));  // stays where it is; the other registers are few
+    }
+}
+
 // ------------------------------------------------------------------- forward
 
 struct StatsEpilogue {
@@ -73,38 +107,27 @@ struct StatsEpilogue {
                                              uint8_t* lds) const {
     f32x2* all = reinterpret_cast<f32x2*>(lds);  // [wave along q][token of the tile]
     const int64_t v0 = row_q + t.q0();
-    const bool whole = row_q + Tl::BQ <= vocab;
+    drop_columns(t, vocab - v0, row_q + Tl::BQ > vocab);
 #pragma unroll
     for (int b = 0; b < Tl::kColumns; ++b) {
       const int64_t token = row_p + t.p0() + kLines * b;
-      const int64_t y = token < tokens ? target[token] : -1;
-      const int64_t rel64 = y - v0;
-      const int rel = rel64 >= 0 && rel64 < Tl::BQ && y < vocab ? (int)rel64 : -1;
-      float m = -INFINITY, hit = 0.0f;
-      bool found = false;
+      float m = -INFINITY;
 #pragma unroll
       for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float z = t.quad(u, b)[i];
-          if (!whole && v0 + kLines * u + i >= vocab) z = -INFINITY;
-          m = fmaxf(m, z);
-          if (rel == kLines * u + i) {
-            hit = z;
-            found = true;
-          }
-        }
-      if (found) z_target[token] = hit;
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, t.quad(u, b)[i]);
       const float at = (m == -INFINITY ? 0.0f : m) * kLog2e;
       float s = 0.0f;
 #pragma unroll
       for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float z = t.quad(u, b)[i];
-          if (!whole && v0 + kLines * u + i >= vocab) z = -INFINITY;
-          s += exp2_hw(fmaf(z, kLog2e, -at));
-        }
+        for (int i = 0; i < 4; ++i) s += exp2_hw(fmaf(t.quad(u, b)[i], kLog2e, -at));
+      const int64_t y = token < tokens ? target[token] : -1;
+      const int rel = column_of<Tl>(y < vocab ? y - v0 : -1);
+      if (__any(rel >= 0)) {
+        const float hit = logit_at(t, b, rel);
+        if (rel >= 0) z_target[token] = hit;
+      }
       // the four lanes that hold this token's logits
       join(m, s, __shfl_xor(m, 16, kWave), __shfl_xor(s, 16, kWave));
       join(m, s, __shfl_xor(m, 32, kWave), __shfl_xor(s, 32, kWave));
@@ -270,30 +293,36 @@ struct ProbEpilogue {
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
                                              uint8_t* lds) const {
     const int64_t v0 = row_q + t.q0();
-    const int left = rows - v0 < Tl::BQ ? (int)(rows - v0) : Tl::BQ;  // columns there are
+    drop_columns(t, rows - v0, row_q + Tl::BQ > rows);
     float h[Tl::kColumns], at[Tl::kColumns];
-    int rel[Tl::kColumns];
 #pragma unroll
     for (int b = 0; b < Tl::kColumns; ++b) {
       const int64_t token = row_p + t.p0() + kLines * b;
       const bool here = token < tokens;
       h[b] = here ? factor[token] : 0.0f;
       at[b] = (here ? lse[token] : 0.0f) * kLog2e;
-      const int64_t r = (here ? target[token] - first : -1) - v0;
-      rel[b] = r >= 0 && r < Tl::BQ ? (int)r : -1;
     }
+    auto p = [&](float z, int b) { return exp2_hw(fmaf(z, kLog2e, -at[b])); };
     t.rows16(
         lds,
         [&](int u, int b) {
-          float v[4];
+          const f32x4 z = t.quad(u, b);
+          const uint32_t lo = Store16<T>::pack(p(z[0], b) * h[b], p(z[1], b) * h[b]);
+          const uint32_t hi = Store16<T>::pack(p(z[2], b) * h[b], p(z[3], b) * h[b]);
+          // a token that takes no part: 0, whatever its logits are
+          return u32x2{h[b] == 0.0f ? 0u : lo, h[b] == 0.0f ? 0u : hi};
+        },
+        [&] {  // 1 off the target's
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int q = kLines * u + i;
-            float p = exp2_hw(fmaf(t.quad(u, b)[i], kLog2e, -at[b]));
-            if (rel[b] == q) p -= 1.0f;
-            v[i] = h[b] != 0.0f && q < left ? p * h[b] : 0.0f;
+          for (int b = 0; b < Tl::kColumns; ++b) {
+            const int64_t token = row_p + t.p0() + kLines * b;
+            const int64_t y = token < tokens ? target[token] - first : -1;
+            const int rel = column_of<Tl>(y < rows ? y - v0 : -1);
+            if (!__any(rel >= 0)) continue;
+            const float z = logit_at(t, b, rel);
+            if (rel >= 0 && h[b] != 0.0f)
+              t.put16(lds, rel, b, (uint16_t)Store16<T>::pack((p(z, b) - 1.0f) * h[b], 0.0f));
           }
-          return u32x2{Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
         },
         [&](int p, int q, u32x4 v) {
           if (row_p + p < tokens) *reinterpret_cast<u32x4*>(d + (row_p + p) * ld + row_q + q) = v;
@@ -335,6 +364,7 @@ struct WeightGradEpilogue {
           const f32x4 v = t.quad(u, b) * f;
           return u32x2{Store16<T>::pack(v[0], v[1]), Store16<T>::pack(v[2], v[3])};
         },
+        [] {},
         [&](int p, int q, u32x4 v) {
           if (row_p + p < rows && row_q + q < hidden)
             *reinterpret_cast<u32x4*>(dw + (row_p + p) * hidden + row_q + q) = v;

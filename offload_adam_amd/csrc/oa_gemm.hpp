@@ -605,17 +605,23 @@ struct Tile {
   // a 264 us product of 4096 x 4096 x 8192 in bf16 and 64 of 280 at 4096 x 14336 x 4096
   // in e4m3.
 
-  // 16-bit results: value(u, b) gives quad u of column b packed into two dwords, and
-  // sink(p, q, v) takes eight consecutive q of one p.
+  // 16-bit results: value(u, b) gives quad u of column b packed into two dwords, amend()
+  // may put16 single ones over them, and sink(p, q, v) takes eight consecutive q of one p.
   static constexpr int kRow16 = BQ * 2 + 16;  // bytes; the odd 16 spread the rows over banks
-  template <class V, class S>
-  __device__ __forceinline__ void rows16(uint8_t* lds, const V& value, const S& sink) const {
+  __device__ __forceinline__ void put16(uint8_t* lds, int rel, int b, uint16_t v) const {
+    *reinterpret_cast<uint16_t*>(lds + (p0() + kLines * b) * kRow16 + (q0() + rel) * 2) = v;
+  }
+  template <class V, class A, class S>
+  __device__ __forceinline__ void rows16(uint8_t* lds, const V& value, const A& amend,
+                                         const S& sink) const {
 #pragma unroll
     for (int b = 0; b < kColumns; ++b)
 #pragma unroll
       for (int u = 0; u < kQuads; ++u)
         *reinterpret_cast<u32x2*>(lds + (p0() + kLines * b) * kRow16 + (q0() + kLines * u) * 2) =
             value(u, b);
+    asm volatile("" ::: "memory");  // amend's stores come after these
+    amend();
     __syncthreads();
     constexpr int lanes = BQ / 8, rows = kThreads / lanes;
     const int q = threadIdx.x % lanes * 8;
