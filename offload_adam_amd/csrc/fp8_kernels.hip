@@ -270,19 +270,35 @@ struct Encoded {
   uint8_t* scales_t; // packed, cols x row blocks
   int64_t ld_t, scale_stride_t;
   float* sums;       // [row block][cols]: sums over 128 rows
+  void* sum;         // [cols], in the type of the source: with one row block, instead
+};
+
+// One or two of them in a launch.
+struct Operands {
+  Source m[2];
+  Encoded e[2];
+  uint32_t blocks_c[2];
+  bool vec[2];
+  uint32_t first;  // workgroups of m[0]
 };
 
 // One workgroup per 128 x 128 block.  4096 x 14336 in bf16 to both kinds of codes: 52
 // us for 235 MB.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_operand_kernel(const Source m, uint32_t blocks_c, bool vec, const Encoded e) {
+fp8_operand_kernel(const Operands all) {
+  const bool second = blockIdx.x >= all.first;
+  const Source m = second ? all.m[1] : all.m[0];
+  const Encoded e = second ? all.e[1] : all.e[0];
+  const uint32_t blocks_c = second ? all.blocks_c[1] : all.blocks_c[0];
+  const uint32_t block = blockIdx.x - (second ? all.first : 0);
+  const bool vec = second ? all.vec[1] : all.vec[0];
   constexpr int kWaves = kThreads / kWave;
   // [column][row], 16-byte pieces of a column at piece ^ (column / 16): lanes that write
   // together meet different banks
   __shared__ __align__(16) uint8_t tile[kBlock][kBlock + 16];
   __shared__ __align__(16) float part[kWaves][kBlock];
-  const int64_t br = blockIdx.x / blocks_c, bc = blockIdx.x % blocks_c;
+  const int64_t br = block / blocks_c, bc = block % blocks_c;
   const int wave = threadIdx.x / kWave, rg = threadIdx.x / 16, cg = threadIdx.x % 16;
   const int r = rg * kPatch, c = cg * kPatch;
   const int64_t r0 = br * kBlock + r, c0 = bc * kBlock + c;
@@ -315,7 +331,7 @@ fp8_operand_kernel(const Source m, uint32_t blocks_c, bool vec, const Encoded e)
       for (int i = 0; i < 4; ++i) a[j + i] = all[i];
     }
   };
-  if (e.sums) {
+  if (e.sums || e.sum) {
     float s[kPatch];
 #pragma unroll
     for (int j = 0; j < kPatch; ++j) {
@@ -327,7 +343,10 @@ fp8_operand_kernel(const Source m, uint32_t blocks_c, bool vec, const Encoded e)
     if (rg == 0) {
 #pragma unroll
       for (int j = 0; j < kPatch; ++j)
-        if (c0 + j < m.cols) e.sums[br * m.cols + c0 + j] = s[j];
+        if (c0 + j < m.cols) {
+          if (e.sum) store1<DT>(e.sum, c0 + j, s[j]);
+          else e.sums[br * m.cols + c0 + j] = s[j];
+        }
     }
     __syncthreads();
   }
@@ -705,10 +724,19 @@ bool vector_rows(const Source& m, int dtype) {
 }
 
 template <int DT>
-int encode_operand(const Source& m, const Encoded& e, hipStream_t s) {
-  const int64_t bc = blocks_of(m.cols), br = blocks_of(m.rows);
-  hipLaunchKernelGGL(fp8_operand_kernel<DT>, dim3((unsigned)(bc * br)), dim3(kThreads), 0, s, m,
-                     (uint32_t)bc, vector_rows(m, DT), e);
+int encode_operands(int count, const Source* const* m, const Encoded* const* e, hipStream_t s) {
+  Operands all{};
+  int64_t blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    all.m[i] = *m[i];
+    all.e[i] = *e[i];
+    all.blocks_c[i] = (uint32_t)blocks_of(m[i]->cols);
+    all.vec[i] = vector_rows(*m[i], DT);
+    blocks += blocks_of(m[i]->cols) * blocks_of(m[i]->rows);
+    if (i == 0) all.first = (uint32_t)blocks;
+  }
+  if (blocks > 0x7FFFFFFF) return OA_ERANGE;
+  hipLaunchKernelGGL(fp8_operand_kernel<DT>, dim3((unsigned)blocks), dim3(kThreads), 0, s, all);
   return launch_status();
 }
 
@@ -811,7 +839,7 @@ struct BackwardPlan {
       x.scales_t = c.take<uint8_t>(blocks_of(tokens) * x.scale_stride_t);
       dw = Output(out_f, in_f, padded_t, c);
     }
-    if (want_db) g.sums = c.take<float>(blocks_of(tokens) * out_f);
+    if (want_db && tokens > kBlock) g.sums = c.take<float>(blocks_of(tokens) * out_f);
     bytes = c.used;
   }
 };
@@ -819,8 +847,11 @@ struct BackwardPlan {
 template <int DT>
 int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* dw, void* db,
              void* ws, hipStream_t s) {
-  const BackwardPlan plan(g.rows, w.in_f, w.out_f, dx != nullptr, dw != nullptr, db != nullptr, ws);
-  int rc = encode_operand<DT>(g, plan.g, s);
+  BackwardPlan plan(g.rows, w.in_f, w.out_f, dx != nullptr, dw != nullptr, db != nullptr, ws);
+  if (!plan.g.sums) plan.g.sum = db;
+  const Source* sources[2] = {&g, &x};
+  const Encoded* codes[2] = {&plan.g, &plan.x};
+  int rc = encode_operands<DT>(dw ? 2 : 1, sources, codes, s);
   if (rc) return rc;
   if (dx) {
     // the weight as it lies: line by line along the outputs, which are summed over
@@ -835,8 +866,6 @@ int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* d
     if (rc) return rc;
   }
   if (dw) {
-    rc = encode_operand<DT>(x, plan.x, s);
-    if (rc) return rc;
     Problem pr{};
     pr.q = Operand{plan.x.qt, plan.x.ld_t, w.in_f, 0};
     pr.p = Operand{plan.g.qt, plan.g.ld_t, w.out_f, 0};
@@ -846,7 +875,7 @@ int backward(const Source& g, const Source& x, const Layer& w, void* dx, void* d
     rc = multiply<DT, true, false>(pr, plan.dw, nullptr, dw, s);
     if (rc) return rc;
   }
-  if (db) {
+  if (plan.g.sums) {
     hipLaunchKernelGGL(fp8_column_sum_kernel<DT>,
                        dim3((unsigned)((w.out_f + kThreads - 1) / kThreads)), dim3(kThreads), 0, s,
                        plan.g.sums, blocks_of(g.rows), w.out_f, db);
