@@ -42,11 +42,13 @@ MODELS = {
 }
 
 
-def build_model(cfg, device):
+def build_model(cfg, device, fused_loss=False):
     import torch
     import torch.nn as nn
     import torch.nn.functional as F
     from torch.utils.checkpoint import checkpoint
+
+    from offload_adam_amd import linear_cross_entropy
 
     class RMSNorm(nn.Module):
         def __init__(self, dim, eps=1e-5):
@@ -98,6 +100,7 @@ def build_model(cfg, device):
         def __init__(self, c):
             super().__init__()
             self.c = c
+            self.fused_loss = fused_loss
             self.embed_tokens = nn.Embedding(c["vocab"], c["hidden"])
             self.layers = nn.ModuleList([Block(c) for _ in range(c["layers"])])
             self.norm = RMSNorm(c["hidden"])
@@ -113,10 +116,12 @@ def build_model(cfg, device):
             for layer in self.layers:
                 x = checkpoint(layer, x, cos, sin, use_reentrant=False)
             x = self.norm(x)
+            tgt = torch.roll(ids, -1, dims=1)
+            if self.fused_loss:  # no logits at all
+                return linear_cross_entropy(x, self.lm_head.weight, tgt)
             # cross-entropy in sequence chunks: the fp32 logits of 4096 x 128256 stay bounded
             loss = x.new_zeros((), dtype=torch.float32)
             chunk = 1024
-            tgt = torch.roll(ids, -1, dims=1)
             for i in range(0, s, chunk):
                 logits = self.lm_head(x[:, i:i + chunk]).float()
                 loss = loss + F.cross_entropy(logits.reshape(-1, logits.shape[-1]),
@@ -331,9 +336,10 @@ class StepCheck:
     # element's row / group / block: the format's largest code error (int8 half of
     # 1/127; int4 one step of 1/8, its largest value is clamped to code 7; NF4 half of
     # the codebook's widest gap, 0.152; NVFP4 half of the 4..6 gap under an e4m3 scale
-    # that may be 1/16 off) plus 2^-8 each for a bf16 scale and the bf16 output
+    # that may be 1/16 off; fp8 half of the 256..288 gap over the smallest largest code of
+    # that range, 1/16) plus 2^-8 each for a bf16 scale and the bf16 output
     QAT_STEP_BOUND = {"Int8QWeight": 0.0125, "Int4QWeight": 0.134, "NF4QWeight": 0.157,
-                      "NVFP4QWeight": 0.19}
+                      "NVFP4QWeight": 0.19, "FP8QWeight": 0.0665}
 
     def __init__(self, torch, model):
         self.torch, self.armed, self.grads, self.sample = torch, False, {}, {}
@@ -516,11 +522,19 @@ class StepCheck:
                                        b.reshape(-1).view(torch.uint8)):
                         report["payload_is_the_encoding_of_the_master"] = False
                         report["failed"].append(f"{name}: payload {key}")
-                span = {"Int8QWeight": master.shape[1], "Int4QWeight": getattr(q, "group_size", 0),
-                        "NF4QWeight": getattr(q, "blocksize", 0), "NVFP4QWeight": 16}[type(q).__name__]
-                grouped = master.reshape(master.shape[0], -1, span)
-                err = (q.dequantize().float().reshape(grouped.shape) - grouped).abs()
-                bound = grouped.abs().amax(dim=-1, keepdim=True) * self.QAT_STEP_BOUND[type(q).__name__]
+                rows = 1
+                if type(q).__name__ == "FP8QWeight":  # blocks of 128 x 128, the last ones short
+                    rows = span = 128
+                else:
+                    span = {"Int8QWeight": master.shape[1],
+                            "Int4QWeight": getattr(q, "group_size", 0),
+                            "NF4QWeight": getattr(q, "blocksize", 0),
+                            "NVFP4QWeight": 16}[type(q).__name__]
+                err, grouped = (
+                    torch.nn.functional.pad(v, (0, -v.shape[1] % span, 0, -v.shape[0] % rows))
+                    .reshape(-(-v.shape[0] // rows), rows, -1, span).abs()
+                    for v in (q.dequantize().float() - master, master))
+                bound = grouped.amax(dim=(1, 3), keepdim=True) * self.QAT_STEP_BOUND[type(q).__name__]
                 if bool((err > bound + 1e-30).any()):
                     report["decoded_payload_within_one_step"] = False
                     report["failed"].append(f"{name}: decoded payload off by more than a step")
@@ -621,12 +635,14 @@ def run(args):
 
     out["link_peak"] = measure_link()
 
-    model = build_model(cfg, dev)
+    model = build_model(cfg, dev, fused_loss=args.fused_loss)
+    out["fused_loss"] = args.fused_loss
     if args.qat:
         from offload_adam_amd import qweight
 
         cls = {"int8": qweight.Int8QWeight, "int4": qweight.Int4QWeight,
-               "nf4": qweight.NF4QWeight, "nvfp4": qweight.NVFP4QWeight}[args.qat]
+               "nf4": qweight.NF4QWeight, "nvfp4": qweight.NVFP4QWeight,
+               "fp8": qweight.FP8QWeight}[args.qat]
         report = qweight.quantize_linears(model, cls, skip_patterns=("lm_head",))
         out["qat"] = {"format": args.qat, "quantized_linears": len(report.quantized),
                       "incompatible": len(report.incompatible),
@@ -869,9 +885,12 @@ def main():
     ap.add_argument("--optimizer", default="offload", choices=["offload", "adam"],
                     help="'adam': the GPU-resident Adam of this package (states in HBM, "
                          "multi-tensor launches in step()) instead of OffloadAdam")
-    ap.add_argument("--qat", default=None, choices=["int8", "int4", "nf4", "nvfp4"],
+    ap.add_argument("--qat", default=None, choices=["int8", "int4", "nf4", "nvfp4", "fp8"],
                     help="quantise every decoder Linear weight (lm_head excluded) and train "
-                         "against fp32 masters: implies --mode fp32_master")
+                         "against fp32 masters: implies --mode fp32_master; fp8 also runs the "
+                         "layers' products on 8-bit codes")
+    ap.add_argument("--fused-loss", action="store_true",
+                    help="linear_cross_entropy instead of logits and cross_entropy")
     ap.add_argument("--grad-cache-gib", type=float, default=None,
                     help="OffloadAdam(grad_cache_bytes=...): HBM for gradients kept on the GPU "
                          "after their write-back (default: the optimizer's; 0 = fetch every time "

@@ -1,11 +1,12 @@
 #!/usr/bin/env python3
 """Per-kernel throughput of everything on the optimizer path besides the fused
 AdamW launch that ``bench.py`` measures: gradient L2 norm, clip coefficient,
-the fused AdamW kernel with the clip coefficient folded in (fp31_master), and
-the eight weight codecs, and the fp32_master step of a quantised weight (fused
-with its re-encoding, and as the reference's two moves).  One JSON line per kernel.
+the fused AdamW kernel with the clip coefficient folded in (fp31_master), the
+weight codecs, the layer on 8-bit codes and the loss of a linear head, and the
+fp32_master step of a quantised weight (fused with its re-encoding, and as the
+reference's two moves).  One JSON line per kernel.
 
-    python bench_kernels.py [--reps 20] [--only norm_large,norm_small,norm_multi,clip,adam,codecs,qat,stream]
+    python bench_kernels.py [--reps 20] [--only norm_large,norm_small,norm_multi,clip,adam,codecs,fp8,products,qat,stream]
 
 Shapes: the offloaded parameters of a Llama-3-8B-shaped decoder for the norm
 and AdamW kernels, one 4096 x 14336 bf16 weight ~N(0, 0.02) with 1 % outliers
@@ -231,6 +232,59 @@ def bench_codecs(args, torch):
     line("dequant_nvfp4_kernel", wl + ", group 16", n * 2.5 + n // 16, us)
 
 
+def bench_products(args, torch):
+    """The linear layer on 8-bit codes and the loss of a linear head, forward and backward,
+    4096 tokens: operations per second, those of the definition counted once (the loss
+    multiplies a quarter more: its backward makes the logits again)."""
+    import torch.nn.functional as F
+
+    from offload_adam_amd import linear_cross_entropy
+    from offload_adam_amd.qweight import FP8QWeight
+
+    def rate(kernel, workload, ops, us):
+        print(json.dumps({"kernel": kernel, "workload": workload, "operations": ops,
+                          "avg_us": round(us, 2), "achieved_TFLOPs": round(ops / us / 1e6, 1),
+                          "bound": "mfma"}), flush=True)
+
+    tokens, vocab, bf16 = 4096, 128256, torch.bfloat16
+    x = torch.randn(tokens, ROWS, device="cuda").to(bf16).requires_grad_(True)
+    w = torch.nn.Parameter(FP8QWeight.from_float(outlier_weight(torch, 0, bf16).t().contiguous()))
+    gy = torch.randn(tokens, COLS, device="cuda").to(bf16)
+
+    def layer(i):
+        torch.autograd.grad(F.linear(x, w), (x, w), gy)
+
+    us = timed(layer, args.reps, torch)
+    rate("F.linear on FP8QWeight, forward and backward", f"{tokens} tokens, {ROWS} -> {COLS}",
+         6 * tokens * ROWS * COLS, us)
+    head = (torch.randn(vocab, ROWS, device="cuda") * 0.02).to(bf16).requires_grad_(True)
+    target = torch.randint(vocab, (tokens,), device="cuda")
+
+    def loss(i):
+        torch.autograd.grad(linear_cross_entropy(x, head, target), (x, head))
+
+    us = timed(loss, args.reps, torch)
+    rate("linear_cross_entropy, forward and backward", f"{tokens} tokens, {ROWS} -> {vocab}",
+         6 * tokens * ROWS * vocab, us)
+
+
+def bench_fp8(args, torch):
+    """The codec of the block-scaled 8-bit weights."""
+    from offload_adam_amd.qweight import _codec_ops as ops
+
+    bf16, slots, n = torch.bfloat16, 5, ROWS * COLS
+    ws = [outlier_weight(torch, i, bf16) for i in range(slots)]
+    wl = f"{ROWS}x{COLS} bf16 weight"
+    q8 = [torch.empty(ROWS, COLS, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(slots)]
+    s8 = [torch.empty(ROWS // 128, COLS // 128, dtype=torch.float8_e8m0fnu, device="cuda")
+          for _ in range(slots)]
+    us = timed(lambda i: ops.quantize_fp8_into(ws[i % slots], q8[i % slots], s8[i % slots]),
+               args.reps, torch)
+    line("fp8_encode_kernel", wl + ", blocks 128 x 128", n * 3 + n // 16384, us)
+    us = timed(lambda i: ops.dequantize_fp8(q8[i % slots], s8[i % slots], bf16), args.reps, torch)
+    line("fp8_decode_kernel", wl + ", blocks 128 x 128", n * 3 + n // 16384, us)
+
+
 def bench_stream_ceiling(args, torch):
     """What a plain device-to-device copy reaches on this part: the runtime's own
     copy kernel (``Tensor.copy_`` between two HBM buffers), reads + writes counted,
@@ -311,9 +365,9 @@ def bench_qat_step(args, torch):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--reps", type=int, default=40)
-    ap.add_argument("--only", default="norm_large,norm_small,norm_multi,clip,adam,codecs,qat,stream",
+    ap.add_argument("--only", default="norm_large,norm_small,norm_multi,clip,adam,codecs,fp8,products,qat,stream",
                     help="comma-separated subset of: norm_large, norm_small, norm_multi, clip, adam, "
-                         "codecs, qat, stream")
+                         "codecs, fp8, products, qat, stream")
     args = ap.parse_args()
 
     import torch
@@ -334,6 +388,10 @@ def main():
         bench_adam_clip(args, torch)
     if "codecs" in todo:
         bench_codecs(args, torch)
+    if "fp8" in todo:
+        bench_fp8(args, torch)
+    if "products" in todo:
+        bench_products(args, torch)
     if "qat" in todo:
         bench_qat_step(args, torch)
     if "stream" in todo:

@@ -395,3 +395,31 @@ def test_a_training_step_through_both_operators():
         master = opt.state[layer.weight]["master_params"].cuda()
         want = FP8QWeight.from_float(master)
         assert torch.equal(_bits(layer.weight.data.weight), _bits(want.weight))
+
+
+def test_the_decoder_of_the_step_benchmark(monkeypatch, capsys):
+    """``bench_e2e.py --qat fp8 --fused-loss``: the loss is that of the logits kept, and the
+    step it follows numerically leaves masters, moments and payloads as they have to be."""
+    import json
+    import sys
+
+    import bench_e2e
+    from offload_adam_amd.qweight import FP8QWeight, quantize_linears
+
+    cfg = bench_e2e.MODELS["tiny"]
+    ids = torch.randint(0, cfg["vocab"], (1, 200), device="cuda")
+    losses = []
+    for fused in (False, True):
+        model = bench_e2e.build_model(cfg, torch.device("cuda:0"), fused_loss=fused)
+        assert quantize_linears(model, FP8QWeight, skip_patterns=("lm_head",)).quantized
+        losses.append(float(model(ids).detach()))
+    # the same weights; the logits kept are rounded to bf16, here under 4 of magnitude
+    assert abs(losses[0] - losses[1]) <= 2 * 4 * 2.0**-8
+    del model
+    monkeypatch.setattr(sys, "argv", ["bench_e2e.py", "--model", "tiny", "--qat", "fp8",
+                                      "--fused-loss", "--check", "--seq", "200", "--steps", "1",
+                                      "--grad-accum", "2"])
+    bench_e2e.main()
+    out = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert out["check"]["passed"], out["check"]
+    assert out["check"]["quantised_tensors"] > 0 and out["qat"]["format"] == "fp8"
