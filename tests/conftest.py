@@ -1,3 +1,4 @@
+import gc
 import sys
 from pathlib import Path
 
@@ -32,6 +33,13 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+def pytest_runtest_setup(item):
+    # tests that compare counts of allocated memory: cycles that earlier tests left behind
+    # are collected before they begin, not while they count
+    if item.module.__name__.endswith("test_zz_no_alloc"):
+        gc.collect()
 
 
 @pytest.fixture(scope="session")
