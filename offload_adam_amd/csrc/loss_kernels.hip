@@ -449,8 +449,9 @@ struct ForwardPlan {
 };
 
 // Elements of d that a piece of the vocabulary may hold: 64 Mi (128 MiB).  A larger
-// piece saves passes over the fp32 sums of dx (one read and write per piece).
-constexpr int64_t kPieceElems = (int64_t)64 << 20;
+// piece saves passes over the fp32 sums of dx (one read and write per piece).  Its rows are
+// limited too: the product for dw addresses 64 lines of d with 32 bits.
+constexpr int64_t kPieceElems = (int64_t)64 << 20, kPieceRows = (int64_t)4 << 20;
 
 struct BackwardPlan {
   int64_t piece;  // vocabulary rows of a piece, whole tiles
@@ -463,6 +464,7 @@ struct BackwardPlan {
     const int64_t whole = up_to(vocab, 256);
     int64_t most = kPieceElems / tokens / 256 * 256;
     if (most < 256) most = 256;
+    if (most > kPieceRows) most = kPieceRows;
     if (most > whole) most = whole;
     piece = up_to(tiles_along(whole, tiles_along(whole, most)), 256);
     dx_cut = cut_for(hidden, tokens, steps_of(piece * 2), true);

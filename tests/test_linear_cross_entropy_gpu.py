@@ -31,8 +31,9 @@ def _inputs(t, h, v, dtype, seed=0, ignore=0.2, ignore_index=-100):
     return x, w, y.cuda()
 
 
-def _expected(x, w, y, grad, reduction, ignore_index=-100):
-    """Everything in 64 bits, and the tolerances."""
+def _expected(x, w, y, grad, reduction, ignore_index=-100, path=256):
+    """Everything in 64 bits, and the tolerances; ``path``: roundings on the way of an
+    exponential into its sum."""
     r = torch.finfo(x.dtype).eps / 2
     hidden = x.shape[1]
     used = y != ignore_index
@@ -42,7 +43,7 @@ def _expected(x, w, y, grad, reduction, ignore_index=-100):
     lse = torch.logsumexp(z, 1)
     at = torch.where(used, y, 0)[:, None]
     each = (lse - z.gather(1, at)[:, 0]) * used
-    tol = (2 * dz + 256 * U + 8 * U * (lse.abs() + z.abs().amax(1))) * used
+    tol = (2 * dz + path * U + 8 * U * (lse.abs() + z.abs().amax(1))) * used
     n = used.sum()
     loss = {"none": each, "sum": each.sum(), "mean": each.sum() / n}[reduction]
     t_sum = tol.sum() + each.abs().sum() * (len(y) + 8) * U
@@ -51,7 +52,7 @@ def _expected(x, w, y, grad, reduction, ignore_index=-100):
     d = torch.exp(z - lse[:, None])
     d.scatter_add_(1, at, torch.full_like(d[:, :1], -1.0))
     # what p = exp(z - lse) is off by before the 1 is taken off, relative to p
-    rel = (dz * 2 + 256 * U + 16 * U * (lse.abs() + z.abs().amax(1)))[:, None]
+    rel = (dz * 2 + path * U + 16 * U * (lse.abs() + z.abs().amax(1)))[:, None]
     p = torch.exp(z - lse[:, None])
     err = (p * rel + d.abs() * (r + 2 * U)) + 2.0**-126  # of d, rounded
     if x.numel() and r == 2.0**-11:  # smallest fp16 step, under the lift of 2^15
@@ -134,6 +135,18 @@ def test_few_tokens_of_a_large_vocabulary(shape):
         want = _expected(x, w, y, grad, reduction)
         for g, e, what in zip(got, want, ("loss", "dx", "dw")):
             _close(g, e, f"{shape} {reduction} {what}")
+
+
+def test_more_rows_than_32_bits_address_in_lines():
+    """64 lines of the logits' gradient of 13 million rows are over 2^30 bytes.  A lane joins
+    13e6 / 128 / 32 pairs, at most 6 roundings each."""
+    x, w, y = _inputs(2, 8, 13_000_000, BF16, seed=2, ignore=0.0)
+    y[1] = 12_999_999
+    grad = _grad_for("none", 2)
+    got = _run(x, w, y, grad, reduction="none")
+    want = _expected(x, w, y, grad, "none", path=6 * 13_000_000 // 128 // 32)
+    for g, e, what in zip(got, want, ("loss", "dx", "dw")):
+        _close(g, e, what)
 
 
 def test_large_logits_and_confident_rows():
