@@ -176,10 +176,13 @@ FP8_BLOCK = 128
 
 def _fp8_payload(codes, scale):
     rows, cols = codes.shape
-    _payload(codes, "weight", torch.float8_e4m3fn, (rows, cols))
-    _payload(scale, "block_scale", torch.float8_e8m0fnu,
-             (-(-rows // FP8_BLOCK), -(-cols // FP8_BLOCK)))
-    if scale.device != codes.device:
+    if not (codes.is_cuda and codes.dtype is torch.float8_e4m3fn and codes.is_contiguous()
+            and scale.dtype is torch.float8_e8m0fnu and scale.is_contiguous()
+            and scale.shape == (-(-rows // FP8_BLOCK), -(-cols // FP8_BLOCK))
+            and scale.device == codes.device):
+        _payload(codes, "weight", torch.float8_e4m3fn, (rows, cols))
+        _payload(scale, "block_scale", torch.float8_e8m0fnu,
+                 (-(-rows // FP8_BLOCK), -(-cols // FP8_BLOCK)))
         raise ValueError("weight and block_scale must be on the same GPU")
     return rows, cols
 
