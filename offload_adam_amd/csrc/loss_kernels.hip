@@ -144,26 +144,49 @@ struct StatsEpilogue {
   }
 };
 
+struct Losses {
+  const float* z_target;
+  const int64_t* target;
+  int64_t tokens, vocab, ignore;
+  float *lse, *loss;  // loss: of every token, or NULL
+
+  // A token whose logits have this maximum and sum: its loss, 0 if it takes no part.  A
+  // target outside [0, vocab) that is not `ignore` makes it NaN.
+  __device__ __forceinline__ float finish(int64_t token, float m, float s, bool& used) const {
+    const float l = m + logf(s);
+    lse[token] = l;
+    const int64_t y = target[token];
+    used = y != ignore;
+    const float v = !used ? 0.0f : y >= 0 && y < vocab ? l - z_target[token] : NAN;
+    if (loss) loss[token] = v;
+    return v;
+  }
+};
+
+// This lane's share of a token's tiles.
+__device__ __forceinline__ void join_tiles(const f32x2* part, int64_t tokens, int64_t token,
+                                           int tiles, int row, float& m, float& s) {
+  m = -INFINITY;
+  s = 0.0f;
+  if (token >= tokens) return;
+#pragma unroll 4
+  for (int j = row; j < tiles; j += kCombineParts) {
+    const f32x2 v = part[(int64_t)j * tokens + token];
+    join(m, s, v[0], v[1]);
+  }
+}
+
 // Joins a token's tiles: 32 lanes per token, eight to a wave, then the lanes (a chain of
 // loads and exponentials is what this takes: 8 us with 8 lanes per token and 125 tiles, 4
-// with 32).  A target outside [0, vocab) that is not `ignore` makes the loss NaN.
+// with 32).
 __global__ void __launch_bounds__(kCombineThreads)
-ce_combine_kernel(const f32x2* __restrict__ part, const float* __restrict__ z_target,
-                  const int64_t* __restrict__ target, int64_t tokens, int64_t vocab,
-                  int64_t ignore, int tiles, float* __restrict__ lse_out,
-                  float* __restrict__ loss_out, float* __restrict__ block_sum,
-                  int* __restrict__ block_count) {
+ce_combine_kernel(const f32x2* __restrict__ part, const Losses a, int tiles,
+                  float* __restrict__ block_sum, int* __restrict__ block_count) {
   __shared__ f32x2 all[kCombineThreads / kWave][kCombineTokens];
   const int col = threadIdx.x % kCombineTokens, row = threadIdx.x / kCombineTokens;
   const int64_t token = (int64_t)blockIdx.x * kCombineTokens + col;
-  float m = -INFINITY, s = 0.0f;
-  if (token < tokens) {
-#pragma unroll 4
-    for (int j = row; j < tiles; j += kCombineParts) {
-      const f32x2 v = part[(int64_t)j * tokens + token];
-      join(m, s, v[0], v[1]);
-    }
-  }
+  float m, s;
+  join_tiles(part, a.tokens, token, tiles, row, m, s);
 #pragma unroll
   for (int off = kCombineTokens; off < kWave; off <<= 1) {
     const float m2 = __shfl_xor(m, off, kWave), s2 = __shfl_xor(s, off, kWave);
@@ -174,15 +197,10 @@ ce_combine_kernel(const f32x2* __restrict__ part, const float* __restrict__ z_ta
   if (threadIdx.x >= kWave) return;
   float loss = 0.0f;
   bool used = false;
-  if (threadIdx.x < kCombineTokens && token < tokens) {
+  if (threadIdx.x < kCombineTokens && token < a.tokens) {
 #pragma unroll
     for (int w = 1; w < kCombineThreads / kWave; ++w) join(m, s, all[w][col][0], all[w][col][1]);
-    const float lse = m + logf(s);
-    lse_out[token] = lse;
-    const int64_t y = target[token];
-    used = y != ignore;
-    if (used) loss = y >= 0 && y < vocab ? lse - z_target[token] : NAN;
-    if (loss_out) loss_out[token] = loss;
+    loss = a.finish(token, m, s, used);
   }
   const float total = wave_sum(loss);
   const int count = __popcll(__ballot(used));
@@ -190,6 +208,40 @@ ce_combine_kernel(const f32x2* __restrict__ part, const float* __restrict__ z_ta
     block_sum[blockIdx.x] = total;
     block_count[blockIdx.x] = count;
   }
+}
+
+// The same and the sum over all tokens, of up to kFewLosses, 32 at a time: one launch
+// instead of two where a launch is what counts.
+constexpr int64_t kFewLosses = 128;
+__global__ void __launch_bounds__(kReduceThreads)
+ce_few_losses_kernel(const f32x2* __restrict__ part, const Losses a, int tiles, int mean,
+                     float* __restrict__ loss_out, float* __restrict__ count_out) {
+  constexpr int kTokens = kReduceThreads / kCombineParts;
+  __shared__ f32x2 all[kReduceThreads / kWave][kTokens];
+  const int col = threadIdx.x % kTokens, row = threadIdx.x / kTokens;
+  float total = 0.0f, count = 0.0f;
+  for (int64_t first = 0; first < a.tokens; first += kTokens) {
+    float m, s;
+    join_tiles(part, a.tokens, first + col, tiles, row, m, s);
+    const float m2 = __shfl_xor(m, kTokens, kWave), s2 = __shfl_xor(s, kTokens, kWave);
+    join(m, s, m2, s2);
+    __syncthreads();
+    if (threadIdx.x % kWave < kTokens) all[threadIdx.x / kWave][col] = f32x2{m, s};
+    __syncthreads();
+    if (row == 0 && first + col < a.tokens) {
+#pragma unroll
+      for (int w = 1; w < kReduceThreads / kWave; ++w) join(m, s, all[w][col][0], all[w][col][1]);
+      bool used;
+      total += a.finish(first + col, m, s, used);
+      count += used ? 1.0f : 0.0f;
+    }
+  }
+  if (threadIdx.x >= kWave) return;
+  total = wave_sum(total);
+  count = wave_sum(count);
+  if (threadIdx.x != 0) return;
+  *count_out = count;
+  *loss_out = mean ? total / count : total;  // nothing took part: 0 / 0
 }
 
 // Sum over the workgroups of the kernel above, in a fixed order, and the number of
@@ -240,35 +292,72 @@ struct TokenFactors {
 };
 constexpr float kF16Lift = 32768.0f;
 
+struct Gradient {
+  const float *grad, *count;
+  const int64_t* target;
+  int64_t tokens, vocab, ignore;
+  int per_token, mean;
+
+  __device__ __forceinline__ bool takes_part(int64_t token) const {
+    return target[token] != ignore;
+  }
+  // NaN for a target that is none
+  __device__ __forceinline__ float fault(int64_t token) const {
+    const int64_t y = target[token];
+    return y < 0 || y >= vocab ? NAN : 0.0f;
+  }
+};
+
+// Factors, and x for dw: rows that take no part become zeros, whatever they hold.  Eight
+// elements of x per lane; without `out`, one token.  Everything but fp16 with one gradient
+// per token, whose factors depend on each other.
+template <class T>
+__global__ void __launch_bounds__(256)
+ce_token_kernel(const Gradient a, const TokenFactors f, const uint16_t* __restrict__ x,
+                int64_t ldx, int64_t hidden, uint16_t* __restrict__ out) {
+  constexpr float kLift = std::is_same<T, F16>::value ? kF16Lift : 1.0f;
+  const int64_t per_row = out ? hidden / 8 : 1;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.tokens * per_row) return;
+  const int64_t token = i / per_row, c = i % per_row * 8;
+  const bool used =
+      a.takes_part(token) && !(a.per_token && a.grad[token] + a.fault(token) == 0.0f);
+  if (c == 0) {
+    float d = 0.0f, dx = 0.0f;
+    if (used) {
+      if (a.per_token) {
+        d = a.grad[token] + a.fault(token);
+        dx = 1.0f;
+      } else {
+        d = kLift + a.fault(token);
+        dx = (a.mean ? a.grad[0] / *a.count : a.grad[0]) / kLift + a.fault(token);
+      }
+    }
+    f.d[token] = d;
+    f.dx[token] = dx;
+  }
+  if (i == 0) {
+    float dw = 1.0f;
+    // no token takes part: 0 times whatever the gradient is
+    if (!a.per_token)
+      dw = *a.count == 0.0f ? 0.0f : (a.mean ? a.grad[0] / *a.count : a.grad[0]) / kLift;
+    *f.dw = dw;
+  }
+  if (!out) return;
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (used) w = *reinterpret_cast<const u32x4*>(x + token * ldx + c);
+  *reinterpret_cast<u32x4*>(out + token * hidden + c) = w;
+}
+
+// fp16, one gradient per token.
 __global__ void __launch_bounds__(kReduceThreads)
-ce_factors_kernel(const float* __restrict__ grad, int per_token, int mean,
-                  const float* __restrict__ count, const int64_t* __restrict__ target,
-                  int64_t tokens, int64_t vocab, int64_t ignore, int f16, TokenFactors f) {
+ce_factors_kernel(const Gradient a, const TokenFactors f) {
   __shared__ float tops[kReduceThreads / kWave];
   float top = 0.0f;
-  const bool one = !per_token && !f16;
-  int used = 0;
-  for (int64_t i = threadIdx.x; i < tokens; i += kReduceThreads) {
-    const int64_t y = target[i];
-    float g = 0.0f;
-    if (y != ignore) {
-      used = 1;
-      g = grad[per_token ? i : 0];
-      if (mean) g = g / *count;
-    }
-    const float bad = y != ignore && (y < 0 || y >= vocab) ? NAN : 0.0f;
-    f.d[i] = (one ? (y != ignore ? 1.0f : 0.0f) : g) + bad;
-    if (!f16) {
-      f.x[i] = y == ignore || (g == 0.0f && bad == 0.0f) ? 0.0f : 1.0f;
-      f.dx[i] = one ? g + bad : f.x[i];
-    }
-    top = fmaxf(top, fabsf(g + bad));
-  }
-  used = __syncthreads_or(used);
-  if (!f16) {
-    // no token: 0 times whatever the gradient is
-    if (threadIdx.x == 0) *f.dw = !one ? 1.0f : !used ? 0.0f : mean ? grad[0] / *count : grad[0];
-    return;
+  for (int64_t i = threadIdx.x; i < a.tokens; i += kReduceThreads) {
+    const float g = a.takes_part(i) ? a.grad[i] + a.fault(i) : 0.0f;
+    f.d[i] = g;
+    top = fmaxf(top, fabsf(g));
   }
   top = wave_max(top);
   if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
@@ -276,7 +365,7 @@ ce_factors_kernel(const float* __restrict__ grad, int per_token, int mean,
   for (int w = 0; w < kReduceThreads / kWave; ++w) top = fmaxf(top, tops[w]);
   if (threadIdx.x == 0) *f.dw = top / kF16Lift;
   // each lane goes over what it wrote itself
-  for (int64_t i = threadIdx.x; i < tokens; i += kReduceThreads) {
+  for (int64_t i = threadIdx.x; i < a.tokens; i += kReduceThreads) {
     const float g = f.d[i];
     int e = 0;
     float m = g == 0.0f ? 0.0f : frexpf(g / top, &e);
@@ -360,6 +449,37 @@ struct SumEpilogue {
   }
 };
 
+// dx itself, where all of it is one product.
+template <class T>
+struct DxEpilogue {
+  uint16_t* dx;
+  int64_t tokens, hidden;
+  const float* factor;
+
+  template <class Tl>
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+                                             uint8_t* lds) const {
+    float f[Tl::kColumns];
+#pragma unroll
+    for (int b = 0; b < Tl::kColumns; ++b) {
+      const int64_t token = row_p + t.p0() + kLines * b;
+      f[b] = token < tokens ? factor[token] : 0.0f;
+    }
+    t.rows16(
+        lds,
+        [&](int u, int b) {
+          const f32x4 v = t.quad(u, b) * f[b];
+          const uint32_t lo = Store16<T>::pack(v[0], v[1]), hi = Store16<T>::pack(v[2], v[3]);
+          return u32x2{f[b] == 0.0f ? 0u : lo, f[b] == 0.0f ? 0u : hi};
+        },
+        [] {},
+        [&](int p, int q, u32x4 v) {
+          if (row_p + p < tokens && row_q + q < hidden)
+            *reinterpret_cast<u32x4*>(dx + (row_p + p) * hidden + row_q + q) = v;
+        });
+  }
+};
+
 template <class T>
 struct WeightGradEpilogue {
   uint16_t* dw;
@@ -412,8 +532,7 @@ __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
   }
 }
 
-// x for dw: each token's row times its factor; rows that take no part become zeros,
-// whatever they hold.  Eight elements per lane.
+// x for dw with factors: rows that take no part become zeros.  Eight elements per lane.
 template <class T>
 __global__ void __launch_bounds__(256)
 ce_x_kernel(const uint16_t* __restrict__ x, int64_t ldx, const float* __restrict__ factor,
@@ -486,7 +605,10 @@ struct BackwardPlan {
     f.dx = c.take<float>(tokens);
     f.dw = c.take<float>(1);
     d = c.take<uint16_t>(tokens * piece);
-    sum = want_dx ? c.take<float>(dx_cut.slices * tokens * hidden) : nullptr;
+    // one piece in one slice is dx as it stands
+    sum = want_dx && (piece < vocab || dx_cut.slices > 1)
+              ? c.take<float>(dx_cut.slices * tokens * hidden)
+              : nullptr;
     x = want_dw ? c.take<uint16_t>(tokens * hidden) : nullptr;
     bytes = c.used;
   }
@@ -515,10 +637,15 @@ int forward(const Head& h, int reduction, float* loss, float* lse, float* count,
     const StatsEpilogue e{h.target, h.tokens, h.vocab, plan.part, plan.z_target};
     int rc = launch_product<T, false, false>(logits_problem(h, 0, h.vocab), plan.cut, e, s);
     if (rc) return rc;
+    const Losses a{plan.z_target, h.target, h.tokens, h.vocab, h.ignore, lse,
+                   reduction == OA_LOSS_NONE ? loss : nullptr};
+    if (reduction != OA_LOSS_NONE && h.tokens <= kFewLosses) {
+      hipLaunchKernelGGL(ce_few_losses_kernel, dim3(1), dim3(kReduceThreads), 0, s, plan.part, a,
+                         plan.tiles, reduction == OA_LOSS_MEAN, loss, count);
+      return launch_status();
+    }
     hipLaunchKernelGGL(ce_combine_kernel, dim3((unsigned)plan.blocks), dim3(kCombineThreads), 0, s,
-                       plan.part, plan.z_target, h.target, h.tokens, h.vocab, h.ignore, plan.tiles,
-                       lse, reduction == OA_LOSS_NONE ? loss : nullptr, plan.block_sum,
-                       plan.block_count);
+                       plan.part, a, plan.tiles, plan.block_sum, plan.block_count);
     rc = launch_status();
     if (rc) return rc;
   }
@@ -533,15 +660,21 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
              const float* grad, uint16_t* dx, uint16_t* dw, void* ws, hipStream_t s) {
   const BackwardPlan plan(h.tokens, h.hidden, h.vocab, dx != nullptr, dw != nullptr, ws);
   const TokenFactors& f = plan.f;
-  hipLaunchKernelGGL(ce_factors_kernel, dim3(1), dim3(kReduceThreads), 0, s, grad,
-                     (int)(reduction == OA_LOSS_NONE), (int)(reduction == OA_LOSS_MEAN), count,
-                     h.target, h.tokens, h.vocab, h.ignore, (int)std::is_same<T, F16>::value, f);
+  const Gradient a{grad, count, h.target, h.tokens, h.vocab, h.ignore,
+                   reduction == OA_LOSS_NONE, reduction == OA_LOSS_MEAN};
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(h.x);
+  const unsigned x_blocks = (unsigned)tiles_along(h.tokens * (dw ? h.hidden / 8 : 1), 256);
+  const bool joint = std::is_same<T, F16>::value && reduction == OA_LOSS_NONE;
+  if (joint)
+    hipLaunchKernelGGL(ce_factors_kernel, dim3(1), dim3(kReduceThreads), 0, s, a, f);
+  else
+    hipLaunchKernelGGL(ce_token_kernel<T>, dim3(x_blocks), dim3(256), 0, s, a, f, x, h.ldx,
+                       h.hidden, plan.x);
   int rc = launch_status();
   if (rc) return rc;
-  if (dw) {
-    hipLaunchKernelGGL(ce_x_kernel<T>, dim3((unsigned)tiles_along(h.tokens * h.hidden / 8, 256)),
-                       dim3(256), 0, s, reinterpret_cast<const uint16_t*>(h.x), h.ldx, f.x,
-                       h.tokens, h.hidden, plan.x);
+  if (joint && dw) {
+    hipLaunchKernelGGL(ce_x_kernel<T>, dim3(x_blocks), dim3(256), 0, s, x, h.ldx, f.x, h.tokens,
+                       h.hidden, plan.x);
     rc = launch_status();
     if (rc) return rc;
   }
@@ -557,8 +690,13 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
       px.q = Operand{h.w + first * h.ldw * 2, h.ldw * 2, h.hidden, rows};
       px.p = Operand{reinterpret_cast<uint8_t*>(plan.d), plan.piece * 2, h.tokens, 0};
       px.k_bytes = (int)(up_to(rows, 8) * 2);
-      const SumEpilogue se{plan.sum, h.tokens, h.hidden, (int)(first == 0)};
-      rc = launch_product<T, true, false>(px, plan.dx_cut, se, s);
+      if (plan.sum) {
+        const SumEpilogue se{plan.sum, h.tokens, h.hidden, (int)(first == 0)};
+        rc = launch_product<T, true, false>(px, plan.dx_cut, se, s);
+      } else {
+        const DxEpilogue<T> de{dx, h.tokens, h.hidden, f.dx};
+        rc = launch_product<T, true, false>(px, plan.dx_cut, de, s);
+      }
       if (rc) return rc;
     }
     if (dw) {
@@ -572,7 +710,7 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
       if (rc) return rc;
     }
   }
-  if (dx) {
+  if (plan.sum) {
     const int64_t quads = h.tokens * h.hidden / 4;
     hipLaunchKernelGGL(ce_dx_kernel<T>, dim3((unsigned)tiles_along(quads, 256)), dim3(256), 0, s,
                        plan.sum, plan.dx_cut.slices, f.dx, h.tokens, h.hidden, dx);

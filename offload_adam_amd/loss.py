@@ -61,22 +61,21 @@ class _LinearCrossEntropy(torch.autograd.Function):
             args, hidden, keep = _head_args(x, w, target, ignore_index, reduction)
             loss = torch.empty((tokens,) if reduction == "none" else (), dtype=torch.float32,
                                device=dev)
-            lse = torch.empty(max(tokens, 1), dtype=torch.float32, device=dev)
-            count = torch.empty(1, dtype=torch.float32, device=dev)
+            stats = torch.empty(tokens + 1, dtype=torch.float32, device=dev)  # lse, count
             if loss.numel():
                 ws = _workspace(dev, tokens, hidden, w.shape[0], 0, 0, 0)
                 code = lib.oa_linear_ce_forward(
-                    *args, loss.data_ptr(), lse.data_ptr(), count.data_ptr(), ws.data_ptr(),
-                    ws.numel(), _lib.current_stream_ptr())
+                    *args, loss.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * tokens,
+                    ws.data_ptr(), ws.numel(), _lib.current_stream_ptr())
                 _lib.check(code, "oa_linear_ce_forward")
-        ctx.save_for_backward(x, weight, target, lse, count)
+        ctx.save_for_backward(x, weight, target, stats)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, target, lse, count = ctx.saved_tensors
+        x, weight, target, stats = ctx.saved_tensors
         want_dx, want_dw = ctx.needs_input_grad[:2]
         tokens, dev = x.shape[0], x.device
         if tokens == 0:
@@ -93,7 +92,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             dw = torch.empty((vocab, hidden), dtype=x.dtype, device=dev) if want_dw else None
             ws = _workspace(dev, tokens, hidden, vocab, 1, int(want_dx), int(want_dw))
             code = lib.oa_linear_ce_backward(
-                *args, lse.data_ptr(), count.data_ptr(), grad.data_ptr(),
+                *args, stats.data_ptr(), stats.data_ptr() + 4 * tokens, grad.data_ptr(),
                 dx.data_ptr() if want_dx else None, dw.data_ptr() if want_dw else None,
                 ws.data_ptr(), ws.numel(), _lib.current_stream_ptr())
             _lib.check(code, "oa_linear_ce_backward")

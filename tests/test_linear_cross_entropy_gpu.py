@@ -251,6 +251,24 @@ def test_one_gradient_at_a_time_gives_the_same_bits():
         assert not linear_cross_entropy(a, b, y).requires_grad
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_tokens_whose_gradient_is_zero(dtype, reduction):
+    """As a caller's own mask makes them: nothing flows, whatever their rows hold."""
+    x, w, y = _inputs(140, 72, 500, dtype, seed=6, ignore=0.0)
+    grad = _grad_for(reduction, 140)
+    if reduction == "none":
+        grad[::3] = 0.0
+        clean = _run(x, w, y, grad, reduction=reduction)
+        x[::3] = float("nan")
+        for a, b in zip(clean[1:], _run(x, w, y, grad, reduction=reduction)[1:]):
+            assert torch.equal(a, b)
+        assert not clean[1][::3].any() and clean[1][1::3].any()
+    else:
+        _, dx, dw = _run(x, w, y, torch.zeros_like(grad), reduction=reduction)
+        assert not dx.any() and not dw.any()
+
+
 def test_gradient_against_differences():
     """Along a direction s of +-1 with steps that 16-bit numbers hold exactly.  The
     third derivative along s is a third cumulant of the logits' direction, at most the
