@@ -193,17 +193,19 @@ __device__ __forceinline__ i32x4 tile_rsrc(const Operand& o, int64_t row0, int t
   return descriptor(o.base + (rows > 0 ? row0 * o.ld : 0) + k, (int)(rows * o.ld));
 }
 
-// The tile of workgroup b: consecutive workgroups go to the 8 XCDs in turn, and
-// each XCD gets one contiguous run of tile numbers, numbered so that a run covers
-// blocks of kGroup tiles along p: the operands of the tiles that an XCD has in
+// Slice and tile of workgroup b of `total`: consecutive workgroups go to the 8 XCDs in
+// turn, and each XCD gets one contiguous run of numbers, slices outermost and tiles so that
+// a run covers blocks of kGroup tiles along p: the operands of the tiles that an XCD has in
 // flight together then come out of its own L2.
 constexpr int kGroup = 8;
-__device__ __forceinline__ void tile_of(uint32_t b, uint32_t tiles_p, uint32_t tiles_q,
-                                        uint32_t& tp, uint32_t& tq) {
-  const uint32_t total = tiles_p * tiles_q;
+__device__ __forceinline__ void tile_of(uint32_t b, uint32_t total, uint32_t tiles_p,
+                                        uint32_t tiles_q, uint32_t& slice, uint32_t& tp,
+                                        uint32_t& tq) {
   const uint32_t per = total / kXcds, extra = total % kXcds;
   const uint32_t x = b % kXcds, j = b / kXcds;
-  const uint32_t id = x * per + (x < extra ? x : extra) + j;
+  uint32_t id = x * per + (x < extra ? x : extra) + j;
+  slice = id / (tiles_p * tiles_q);
+  id -= slice * tiles_p * tiles_q;
   const uint32_t group = id / (kGroup * tiles_q);
   const uint32_t first = group * kGroup;
   const uint32_t wide = tiles_p - first < kGroup ? tiles_p - first : kGroup;
@@ -760,10 +762,8 @@ template <class T, class E>
 __global__ void __launch_bounds__(T::kThreads) product_kernel(const Problem pr, const E epilogue) {
   __shared__ __align__(16) uint8_t lds[T::kLdsBytes];
   T t;
-  uint32_t tp, tq;
-  const uint32_t tiles = pr.tiles_p * pr.tiles_q;
-  const uint32_t slice = blockIdx.x / tiles;
-  tile_of(blockIdx.x - slice * tiles, pr.tiles_p, pr.tiles_q, tp, tq);
+  uint32_t slice, tp, tq;
+  tile_of(blockIdx.x, gridDim.x, pr.tiles_p, pr.tiles_q, slice, tp, tq);
   const int64_t row_q = (int64_t)tq * T::BQ, row_p = (int64_t)tp * T::BP;
   const int steps = (pr.k_bytes + kStepBytes - 1) / kStepBytes;
   const int step0 = (int)slice * pr.steps_per_slice;
