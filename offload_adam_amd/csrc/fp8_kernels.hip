@@ -10,7 +10,9 @@
 //   dx = gq wq       gq: blocks of 1 x 128 along the outputs     (T x N) (N x K)
 //   dw = gt^T xt     gt, xt: blocks of 128 x 1 along the tokens  (T x N)^T (T x K)
 //
-// Products accumulate in fp32 and are rounded once, to the type of x.
+// Products accumulate in fp32 and are rounded once, to the type of x.  4096 tokens, 4096 ->
+// 14336, bf16: forward 13 us to encode x and 207 to 227 for y (2.1 to 2.3 PFLOP/s); backward
+// 59 to encode, 175 to 200 for dx, 193 to 240 for dw, by the clock that power allows.
 
 #include <math.h>
 
@@ -190,7 +192,9 @@ __device__ __forceinline__ void drop_infinities(float (&v)[kPatch][kPatch]) {
 
 // -------------------------------------------------------------- weight codec
 
-// One workgroup per 128 x 128 block: one read of the source, one write of the codes.
+// One workgroup per 128 x 128 block: one read of the source, one write of the codes.  Bound
+// by HBM: 14336 x 4096, 57 us from fp32 (293 MB), 27 from bf16 (176 MB, part of them still
+// in the memory-side cache).
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 fp8_encode_kernel(const Source m, uint32_t blocks_c, bool vec, uint8_t* __restrict__ q,
@@ -234,7 +238,8 @@ __device__ __forceinline__ void decode4(uint32_t w, float s, float* x) {
   x[3] = b[1] * s;
 }
 
-// 16 codes per lane (cols is a multiple of 16: one row, one block).
+// 16 codes per lane (cols is a multiple of 16: one row, one block).  14336 x 4096 to bf16:
+// 28 us for 176 MB.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 fp8_decode_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scales, int64_t rows,
@@ -398,7 +403,8 @@ fp8_operand_kernel(const Operands all) {
 }
 
 // The row operand alone (codes in blocks of 1 x 128 along the columns): 16 lanes to a
-// block, eight elements to a lane, columns from `cols` up to e.ld zero.
+// block, eight elements to a lane, columns from `cols` up to e.ld zero.  4096 x 4096 in bf16:
+// 13 us for 50 MB; 16384 x 14336: 130 us for 705 MB.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 fp8_rows_kernel(const Source m, bool vec, const Encoded e) {
