@@ -422,7 +422,7 @@ int oa_quant_fp8(const void* src, int src_dtype, int64_t src_row_stride, int64_t
 int oa_dequant_fp8(const void* q, const void* scales, int64_t rows, int64_t cols, void* out,
                    int out_dtype, int64_t out_row_stride, void* stream);
 
-/* 0 for sizes that are not positive.  backward = 0: want_* unused. */
+/* 0 for sizes out of range.  backward = 0: want_* unused. */
 size_t oa_fp8_linear_workspace_bytes(int64_t tokens, int64_t in_features,
                                      int64_t out_features, int backward, int want_dx,
                                      int want_dw, int want_db);

@@ -984,6 +984,7 @@ extern "C" size_t oa_fp8_linear_workspace_bytes(int64_t tokens, int64_t in_featu
                                                 int64_t out_features, int backward, int want_dx,
                                                 int want_dw, int want_db) {
   if (tokens <= 0 || in_features <= 0 || out_features <= 0) return 0;
+  if (tokens > kMostRows || in_features > kMostRows || out_features > kMostRows) return 0;
   if (!backward) {
     const bool few = takes_few(Layer{nullptr, nullptr, out_features, in_features}, tokens);
     return ForwardPlan(tokens, in_features, out_features, few, nullptr).bytes;

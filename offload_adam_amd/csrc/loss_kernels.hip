@@ -725,17 +725,20 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
   return rc;
 }
 
+constexpr int64_t kMostTokens = 1 << 22, kMostHidden = 1 << 20, kMostVocab = 1 << 24;
+
 int check_head(const Head& h, int dtype, int reduction) {
   if (dtype != OA_BF16 && dtype != OA_F16) return OA_EINVAL;
   if (reduction != OA_LOSS_NONE && reduction != OA_LOSS_MEAN && reduction != OA_LOSS_SUM)
     return OA_EINVAL;
   if (h.tokens < 0 || h.hidden <= 0 || h.vocab <= 0 || !h.w) return OA_EINVAL;
   if (h.tokens > 0 && (!h.x || !h.target)) return OA_EINVAL;
-  if (h.ldw < h.hidden || (h.tokens > 1 && h.ldx < h.hidden)) return OA_EINVAL;
+  if (h.ldw < h.hidden || h.ldx < h.hidden) return OA_EINVAL;
   if (h.hidden % 8 || h.ldx % 8 || h.ldw % 8 || !aligned_to(h.x, 16) || !aligned_to(h.w, 16) ||
       !aligned_to(h.target, 8))
     return OA_EALIGN;
-  if (h.ldx > (1 << 20) || h.ldw > (1 << 20) || h.tokens > (1 << 22) || h.vocab > (1 << 24))
+  if (h.ldx > kMostHidden || h.ldw > kMostHidden || h.tokens > kMostTokens ||
+      h.vocab > kMostVocab)
     return OA_ERANGE;
   return 0;
 }
@@ -748,6 +751,7 @@ using namespace oa;
 extern "C" size_t oa_linear_ce_workspace_bytes(int64_t tokens, int64_t hidden, int64_t vocab,
                                                int backward, int want_dx, int want_dw) {
   if (tokens < 0 || hidden <= 0 || vocab <= 0) return 0;
+  if (tokens > kMostTokens || hidden > kMostHidden || vocab > kMostVocab) return 0;
   // never 0: the workspace of an empty batch is a valid pointer too
   if (!backward) return ForwardPlan(tokens, hidden, vocab, nullptr).bytes + 256;
   if (tokens == 0) return 0;

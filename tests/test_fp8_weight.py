@@ -199,3 +199,6 @@ def test_the_c_entry_points_refuse_before_any_launch():
     assert bwd(dx=None, dw=None, db=None) == -1 and bwd(g=None) == -1 and bwd(ldg=4) == -1
     assert bwd(dx=odd) == -2 and bwd(dw=odd) == -2 and bwd(db=odd) == -2
     assert lib.oa_fp8_linear_workspace_bytes(0, 16, 16, 0, 0, 0, 0) == 0
+    for sizes in ((1 << 40, 1 << 40, 16), (4, 1 << 62, 16), (4, 16, (1 << 22) + 1)):
+        assert lib.oa_fp8_linear_workspace_bytes(*sizes, 0, 0, 0, 0) == 0
+        assert lib.oa_fp8_linear_workspace_bytes(*sizes, 1, 1, 1, 1) == 0

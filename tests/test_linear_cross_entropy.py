@@ -60,6 +60,7 @@ def test_the_c_entry_points_refuse_before_any_launch():
         assert f(t=-1) == -1 and f(h=0) == -1 and f(v=0) == -1
         assert f(x=None) == -1 and f(w=None) == -1 and f(y=None) == -1 and f(ws=None) == -1
         assert f(ldx=8) == -1 and f(ldw=8) == -1  # shorter than a row
+        assert f(t=1, ldx=8) == -1
         assert f(h=12, ldx=16, ldw=16) == -2 and f(ldx=20) == -2 and f(ldw=20) == -2
         assert f(x=odd) == -2 and f(w=odd) == -2 and f(ws=odd) == -2
         assert f(ldx=1 << 21) == -3 and f(t=(1 << 22) + 1) == -3 and f(v=(1 << 24) + 1) == -3
@@ -68,6 +69,9 @@ def test_the_c_entry_points_refuse_before_any_launch():
     assert bwd(t=0) == -1 and bwd(grad=None) == -1 and bwd(dx=None, dw=None) == -1
     assert bwd(dx=odd) == -2
     assert lib.oa_linear_ce_workspace_bytes(-1, 16, 10, 0, 0, 0) == 0
+    for sizes in ((1 << 40, 16, 1 << 40), (4, 1 << 62, 10), (4, 16, (1 << 24) + 1)):
+        for backward in (0, 1):
+            assert lib.oa_linear_ce_workspace_bytes(*sizes, backward, 1, 1) == 0
     assert lib.oa_linear_ce_workspace_bytes(0, 16, 10, 0, 0, 0) > 0
     # a backward pass holds far less than the logits of the 8B model's micro-batch in fp32
     assert lib.oa_linear_ce_workspace_bytes(4096, 4096, 128256, 1, 1, 1) < 4096 * 128256 * 4 // 3
