@@ -40,6 +40,10 @@ __device__ __forceinline__ float load1(const void* base, int64_t i) {
   return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
+// 16 bytes that are aligned to an element only: one access all the same.
+typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+
 // Eight elements as they lie in memory.
 template <int DT>
 struct Octet {
@@ -47,20 +51,19 @@ struct Octet {
   u32x4 w[kWords];
 
   __device__ __forceinline__ void load(const void* base, int64_t i) {
-    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(base) +
-                                                    i * (DT == OA_F32 ? 4 : 2));
+    const uint8_t* p = static_cast<const uint8_t*>(base) + i * (DT == OA_F32 ? 4 : 2);
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) w[k] = p[k];
+    for (int k = 0; k < kWords; ++k) {
+      if (DT == OA_F32)
+        w[k] = __builtin_bit_cast(u32x4, f32x4(*reinterpret_cast<const f32x4_4*>(p + 16 * k)));
+      else
+        w[k] = *reinterpret_cast<const u32x4_2*>(p + 16 * k);
+    }
   }
   __device__ __forceinline__ float operator[](int k) const {
     if (DT == OA_F32) return __uint_as_float(w[k / 4 % kWords][k % 4]);
     const uint16_t h = (uint16_t)(w[0][k / 2 % 4] >> (16 * (k % 2)));
     return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-  }
-  // element k of a row that is loaded piece by piece; the octet starts as zeros
-  __device__ __forceinline__ void put(int k, const void* base, int64_t i) {
-    if (DT == OA_F32) w[k / 4 % kWords][k % 4] = static_cast<const uint32_t*>(base)[i];
-    else w[0][k / 2 % 4] |= (uint32_t)static_cast<const uint16_t*>(base)[i] << (16 * (k % 2));
   }
 };
 
@@ -135,20 +138,22 @@ __device__ __forceinline__ float max_of_16(float v) {
 
 // One lane's 8 x 8 patch of block (br, bc): rows r .. r+7, columns c .. c+7 of it; what lies
 // outside the source reads as zero.  `vec`: rows are 16-byte aligned, whole octets, and
-// 128 of them span less than 2^31 bytes.
+// 128 of them span less than 2^31 bytes.  Else an octet is one load that may cross a line,
+// and the last one of a row, if it is not whole, eight: a gradient of 5064 x 14085 in fp16
+// to both kinds of codes takes 64 us, 91 with single elements throughout; 5064 x 14080, 59.
 template <int DT>
 __device__ __forceinline__ void load_patch(const Source& m, int64_t br, int64_t bc, int r, int c,
                                            bool vec, float (&v)[kPatch][kPatch]) {
   constexpr int kSize = DT == OA_F32 ? 4 : 2;
   const int64_t first = br * kBlock, left = m.rows - first, c0 = bc * kBlock + c;
   const int rows = left < kBlock ? (int)left : kBlock;
+  Octet<DT> o[kPatch];
   if (vec) {
     const uint8_t* base = static_cast<const uint8_t*>(m.base) + first * m.stride * kSize;
     const int pitch = (int)m.stride * kSize;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(base), 0, (rows - 1) * pitch + (int)m.cols * kSize, 0x00020000);
     const int at = c0 < m.cols ? r * pitch + (int)c0 * kSize : kOut;
-    Octet<DT> o[kPatch];
 #pragma unroll
     for (int p = 0; p < kPatch; ++p)
 #pragma unroll
@@ -160,17 +165,23 @@ __device__ __forceinline__ void load_patch(const Source& m, int64_t br, int64_t 
     for (int p = 0; p < kPatch; ++p)
 #pragma unroll
       for (int j = 0; j < kPatch; ++j) v[p][j] = o[p][j];
+  } else if (c0 + kPatch <= m.cols) {
+    // rows past the end: some row that is there, and zeros in its place
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p)
+      o[p].load(m.base, (first + (r + p < rows ? r + p : 0)) * m.stride + c0);
+#pragma unroll
+    for (int p = 0; p < kPatch; ++p)
+#pragma unroll
+      for (int j = 0; j < kPatch; ++j) v[p][j] = r + p < rows ? o[p][j] : 0.0f;
   } else {
 #pragma unroll
-    for (int p = 0; p < kPatch; ++p) {
-      const int64_t row = (first + (r + p < rows ? r + p : 0)) * m.stride;
+    for (int p = 0; p < kPatch; ++p)
 #pragma unroll
-      for (int j = 0; j < kPatch; ++j) {
-        const bool in = r + p < rows && c0 + j < m.cols;
-        const float x = load1<DT>(m.base, row + (c0 + j < m.cols ? c0 + j : 0));
-        v[p][j] = in ? x : 0.0f;
-      }
-    }
+      for (int j = 0; j < kPatch; ++j)
+        v[p][j] = r + p < rows && c0 + j < m.cols
+                      ? load1<DT>(m.base, (first + r + p) * m.stride + c0 + j)
+                      : 0.0f;
   }
 }
 
@@ -407,19 +418,13 @@ fp8_operand_kernel(const Operands all) {
 // 13 us for 50 MB; 16384 x 14336: 130 us for 705 MB.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_rows_kernel(const Source m, bool vec, const Encoded e) {
+fp8_rows_kernel(const Source m, const Encoded e) {
   const int64_t per_row = e.ld / kPatch;
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t r = i / per_row, c = i % per_row * kPatch;
   if (r >= m.rows) return;  // 16 lanes together: rows are whole blocks long
   float x[kPatch] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (vec) {
-    if (c < m.cols) load8<DT>(m.base, r * m.stride + c, x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kPatch; ++j)
-      if (c + j < m.cols) x[j] = load1<DT>(m.base, r * m.stride + c + j);
-  }
+  if (c < m.cols) load8<DT>(m.base, r * m.stride + c, x);  // whole octets
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < kPatch; ++j) {
@@ -448,13 +453,14 @@ fp8_column_sum_kernel(const float* __restrict__ sums, int64_t blocks_r, int64_t 
 
 // ------------------------------------------------------------------ products
 
-// The product, plus the bias of its columns, in the caller's type.
+// The product, plus the bias of its columns, in the caller's type.  Whole octets of a row
+// are one store, aligned or not: 5064 x 14085 x 240 takes 52 us, 136 with single elements
+// for rows that are not aligned; 5064 x 14080 x 240, 47.
 template <int DT>
 struct StoreEpilogue {
   void* out;
   int64_t rows, cols;  // p, q
   const void* bias;    // by q, or NULL
-  bool vec;            // rows of the result are 16-byte aligned, whole octets
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
@@ -474,7 +480,7 @@ struct StoreEpilogue {
       t.rows32(lds, [&](int p, int q, f32x4 v) {
         if (row_p + p >= rows) return;
         float* o = static_cast<float*>(out) + (row_p + p) * cols + row_q + q;
-        if (vec && row_q + q < cols) *reinterpret_cast<f32x4*>(o) = v;
+        if (row_q + q + 4 <= cols) *reinterpret_cast<f32x4_4*>(o) = v;
         else
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -491,7 +497,7 @@ struct StoreEpilogue {
           [&](int p, int q, u32x4 v) {
             if (row_p + p >= rows) return;
             uint16_t* o = static_cast<uint16_t*>(out) + (row_p + p) * cols + row_q + q;
-            if (vec && row_q + q < cols) *reinterpret_cast<u32x4*>(o) = v;
+            if (row_q + q + 8 <= cols) *reinterpret_cast<u32x4_2*>(o) = v;
             else
 #pragma unroll
               for (int i = 0; i < 8; ++i)
@@ -505,12 +511,11 @@ struct StoreEpilogue {
 struct SliceEpilogue {
   float* out;
   int64_t rows, cols;
-  bool vec;
 
   template <class Tl>
   __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq,
                                              int slice, uint8_t* lds) const {
-    const StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr, vec};
+    const StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr};
     e(t, row_q, row_p, tq, 0, lds);
   }
 };
@@ -527,7 +532,6 @@ struct Few {
   int64_t out_f;
   int in_f, blocks_k;
   Source x;            // ENCODE
-  bool vec;
   const uint8_t *xq, *xs;  // else
   int64_t ldx;         // of the codes
   int64_t xs_stride;
@@ -569,14 +573,7 @@ __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) 
       const int token = i / per_row, c = i % per_row * kPatch;
       x[j] = Octet<DT>{};
       if (token >= a.tokens) continue;
-      const int64_t at = token * a.x.stride + c;
-      if (a.vec) {
-        if (c < a.in_f) x[j].load(a.x.base, at);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kPatch; ++e)
-          if (c + e < a.in_f) x[j].put(e, a.x.base, at + e);
-      }
+      if (c < a.in_f) x[j].load(a.x.base, token * a.x.stride + c);
     }
   }
   auto fetch = [&](int step, i32x8& q, int& sq, i32x8 (&p)[TILES], int (&sp)[TILES]) {
@@ -711,10 +708,10 @@ template <int DT, bool Q_PACKED, bool Q_LINES>
 int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hipStream_t s) {
   typedef E4m3<Q_PACKED> T;
   if (o.cut.slices == 1) {
-    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias, o.cols % 8 == 0 && aligned_to(out, 16)};
+    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias};
     return launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
   }
-  const SliceEpilogue e{o.part, o.rows, o.cols, o.cols % 4 == 0};
+  const SliceEpilogue e{o.part, o.rows, o.cols};
   int rc = launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
   if (rc) return rc;
   const int64_t count = o.rows * o.cols;
@@ -750,7 +747,7 @@ template <int DT>
 int encode_rows(const Source& m, const Encoded& e, hipStream_t s) {
   const int64_t lanes = m.rows * (e.ld / kPatch);
   hipLaunchKernelGGL(fp8_rows_kernel<DT>, dim3((unsigned)((lanes + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, s, m, vector_rows(m, DT), e);
+                     dim3(kThreads), 0, s, m, e);
   return launch_status();
 }
 
@@ -797,7 +794,7 @@ int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws
   if (few) {
     const int waves = few_waves(w), tokens = (int)x.rows;
     const Few<DT> a{w.q, w.scales, w.out_f, (int)w.in_f, (int)blocks_of(w.in_f),
-                    x, vector_rows(x, DT), plan.x.q, plan.x.scales, plan.x.ld,
+                    x, plan.x.q, plan.x.scales, plan.x.ld,
                     plan.x.scale_stride, tokens, bias, y};
     if (tokens <= kFewEncodeTokens && tokens * plan.x.ld <= kFewCodes) {
       launch_few<DT, 1, true>(a, waves, s);
