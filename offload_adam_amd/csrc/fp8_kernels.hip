@@ -40,8 +40,9 @@ __device__ __forceinline__ float load1(const void* base, int64_t i) {
   return DT == OA_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
 }
 
-// 16 bytes that are aligned to an element only: one access all the same.
+// Vectors that are aligned to an element only: one access all the same.
 typedef uint32_t u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Eight elements as they lie in memory.
@@ -463,7 +464,7 @@ struct StoreEpilogue {
   const void* bias;    // by q, or NULL
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place&,
                                              uint8_t* lds) const {
     if (bias) {
 #pragma unroll
@@ -507,16 +508,27 @@ struct StoreEpilogue {
   }
 };
 
-// One slice of a product split along k: fp32, [slice][row][cols].
-struct SliceEpilogue {
-  float* out;
-  int64_t rows, cols;
+// The same where some tiles are cut along k: their slices go to fp32 tiles of their own,
+// [number of the tile][slice][row][column], with as many rows as there are when those are
+// less than a tile's.
+template <int DT>
+struct CutEpilogue {
+  StoreEpilogue<DT> whole;
+  float* part;
+  int slices, area;  // of a slice's tile, elements
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq,
-                                             int slice, uint8_t* lds) const {
-    const StoreEpilogue<OA_F32> e{out + (int64_t)slice * rows * cols, rows, cols, nullptr};
-    e(t, row_q, row_p, tq, 0, lds);
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p,
+                                             const Place& place, uint8_t* lds) const {
+    if (place.slice < 0) {
+      whole(t, row_q, row_p, place, lds);
+      return;
+    }
+    float* out = part + ((int64_t)place.number * slices + place.slice) * area;
+    t.rows32(lds, [&](int p, int q, f32x4 v) {
+      if (row_p + p < whole.rows && row_q + q < whole.cols)
+        *reinterpret_cast<f32x4*>(out + p * Tl::BQ + q) = v;
+    });
   }
 };
 
@@ -679,44 +691,70 @@ void launch_few(const Few<DT>& a, int waves, hipStream_t s) {
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 16, ENCODE>), grid, block, 0, s, a);
 }
 
+// Slices of the cut tiles -> results, four columns of a row per lane.
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-fp8_join_kernel(const float* __restrict__ part, int slices, int64_t count, int64_t cols,
-                const void* __restrict__ bias, void* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= count) return;
-  float v = part[i];
+fp8_join_kernel(const CutEpilogue<DT> e, int side, uint32_t first, uint32_t tiles_p,
+                uint32_t tiles_q) {
+  const uint32_t per_tile = (uint32_t)((e.area / 4 + kThreads - 1) / kThreads);
+  const uint32_t number = blockIdx.x / per_tile;
+  const int i = (int)((blockIdx.x - number * per_tile) * kThreads + threadIdx.x) * 4;
+  uint32_t tp, tq;
+  tile_at(first + number, tiles_p, tiles_q, tp, tq);
+  const int64_t row = (int64_t)tp * side + i / side, col = (int64_t)tq * side + i % side;
+  if (i >= e.area || row >= e.whole.rows || col >= e.whole.cols) return;
+  const float* part = e.part + (int64_t)number * e.slices * e.area + i;
+  f32x4 v = *reinterpret_cast<const f32x4*>(part);
 #pragma unroll 8
-  for (int s = 1; s < slices; ++s) v += part[s * count + i];
-  if (bias) v += load1<DT>(bias, i % cols);
-  store1<DT>(out, i, v);
+  for (int s = 1; s < e.slices; ++s)
+    v += *reinterpret_cast<const f32x4*>(part + (int64_t)s * e.area);
+  const int64_t at = row * e.whole.cols + col;
+  const int left = e.whole.cols - col < 4 ? (int)(e.whole.cols - col) : 4;
+  if (e.whole.bias) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) v[k] += load1<DT>(e.whole.bias, col + k);
+  }
+  if (left < 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < left) store1<DT>(e.whole.out, at + k, v[k]);
+  } else if constexpr (DT == OA_F32) {
+    *reinterpret_cast<f32x4_4*>(static_cast<float*>(e.whole.out) + at) = v;
+  } else {
+    *reinterpret_cast<u32x2_2*>(static_cast<uint16_t*>(e.whole.out) + at) =
+        u32x2{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3])};
+  }
 }
 
 // A product's rows and columns, how it is cut, and the partial sums of its slices.
 struct Output {
-  int64_t rows = 0, cols = 0;
-  Cut cut{false, 1};
+  int64_t rows = 0, cols = 0, tiles_p = 0, tiles_q = 0, side = 0;
+  Cut cut{false, 1, 0};
   float* part = nullptr;
   Output() {}
   Output(int64_t rows_, int64_t cols_, int64_t k_bytes, Carver& c) : rows(rows_), cols(cols_) {
-    cut = cut_for(cols, rows, steps_of(k_bytes), true);
-    if (cut.slices > 1) part = c.take<float>(cut.slices * rows * cols);
+    cut = cut_for(cols, rows, steps_of(k_bytes), kLastTiles);
+    side = cut.large ? 256 : 128;
+    tiles_p = tiles_along(rows, side);
+    tiles_q = tiles_along(cols, side);
+    if (cut.slices > 1) part = c.take<float>(cut_tiles() * cut.slices * area());
   }
+  int64_t cut_tiles() const { return tiles_p * tiles_q - cut.whole; }
+  int64_t area() const { return side * (rows < side ? rows : side); }
 };
 
 template <int DT, bool Q_PACKED, bool Q_LINES>
 int multiply(const Problem& pr, const Output& o, const void* bias, void* out, hipStream_t s) {
   typedef E4m3<Q_PACKED> T;
-  if (o.cut.slices == 1) {
-    const StoreEpilogue<DT> e{out, o.rows, o.cols, bias};
-    return launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
-  }
-  const SliceEpilogue e{o.part, o.rows, o.cols};
+  const StoreEpilogue<DT> whole{out, o.rows, o.cols, bias};
+  if (o.cut.slices == 1) return launch_product<T, Q_LINES, false>(pr, o.cut, whole, s);
+  const CutEpilogue<DT> e{whole, o.part, o.cut.slices, (int)o.area()};
   int rc = launch_product<T, Q_LINES, false>(pr, o.cut, e, s);
   if (rc) return rc;
-  const int64_t count = o.rows * o.cols;
-  hipLaunchKernelGGL(fp8_join_kernel<DT>, dim3((unsigned)((count + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, s, o.part, o.cut.slices, count, o.cols, bias, out);
+  const int64_t blocks = o.cut_tiles() * tiles_along(o.area() / 4, kThreads);
+  hipLaunchKernelGGL(fp8_join_kernel<DT>, dim3((unsigned)blocks), dim3(kThreads), 0, s, e,
+                     (int)o.side, (uint32_t)o.cut.whole, (uint32_t)o.tiles_p, (uint32_t)o.tiles_q);
   return launch_status();
 }
 

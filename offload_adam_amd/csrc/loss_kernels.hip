@@ -107,7 +107,7 @@ struct StatsEpilogue {
   float* z_target;  // [token]
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int tq, int,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place& place,
                                              uint8_t* lds) const {
     f32x2* all = reinterpret_cast<f32x2*>(lds);  // [wave along q][token of the tile]
     const int64_t v0 = row_q + t.q0();
@@ -143,7 +143,7 @@ struct StatsEpilogue {
       float m = v[0], s = v[1];
 #pragma unroll
       for (int w = 1; w < Tl::kWavesQ; ++w) join(m, s, all[w * Tl::BP + i][0], all[w * Tl::BP + i][1]);
-      if (row_p + i < tokens) part[(int64_t)tq * tokens + row_p + i] = f32x2{m, s};
+      if (row_p + i < tokens) part[(int64_t)place.tq * tokens + row_p + i] = f32x2{m, s};
     }
   }
 };
@@ -397,7 +397,7 @@ struct ProbEpilogue {
   int64_t ld;
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place&,
                                              uint8_t* lds) const {
     const int64_t v0 = row_q + t.q0();
     drop_columns(t, rows - v0, row_q + Tl::BQ > rows);
@@ -444,9 +444,9 @@ struct SumEpilogue {
   int first;  // nothing is there yet
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int slice,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place& place,
                                              uint8_t* lds) const {
-    float* base = sum + ((int64_t)slice * tokens + row_p) * hidden + row_q;
+    float* base = sum + ((int64_t)place.slice * tokens + row_p) * hidden + row_q;
     t.rows32(lds, [&](int p, int q, f32x4 v) {
       if (row_p + p >= tokens || row_q + q >= hidden) return;  // hidden is a multiple of 8
       f32x4* o = reinterpret_cast<f32x4*>(base + p * hidden + q);
@@ -463,7 +463,7 @@ struct DxEpilogue {
   const float* factor;
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place&,
                                              uint8_t* lds) const {
     float f[Tl::kColumns];
 #pragma unroll
@@ -493,7 +493,7 @@ struct WeightGradEpilogue {
   const float* factor;
 
   template <class Tl>
-  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, int, int,
+  __device__ __forceinline__ void operator()(Tl& t, int64_t row_q, int64_t row_p, const Place&,
                                              uint8_t* lds) const {
     const float f = *factor;
     t.rows16(
@@ -573,7 +573,7 @@ struct ForwardPlan {
   int* block_count;
   size_t bytes;
   ForwardPlan(int64_t tokens, int64_t hidden, int64_t vocab, void* ws) {
-    cut = cut_for(vocab, tokens > 0 ? tokens : 1, steps_of(hidden * 2), false);
+    cut = cut_for(vocab, tokens > 0 ? tokens : 1, steps_of(hidden * 2), kNoSlices);
     tiles = (int)tiles_along(vocab, cut.large ? 256 : 128);
     blocks = (int)tiles_along(tokens, kCombineTokens);
     Carver c{static_cast<uint8_t*>(ws)};
@@ -604,7 +604,7 @@ struct BackwardPlan {
     if (most > kPieceRows) most = kPieceRows;
     if (most > whole) most = whole;
     piece = up_to(tiles_along(whole, tiles_along(whole, most)), 256);
-    dx_cut = cut_for(hidden, tokens, steps_of(piece * 2), true);
+    dx_cut = cut_for(hidden, tokens, steps_of(piece * 2), kAllTiles);
     Carver c{static_cast<uint8_t*>(ws)};
     f.d = c.take<float>(tokens);
     f.x = c.take<float>(tokens);
@@ -688,7 +688,7 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
     const int64_t rows = h.vocab - first < plan.piece ? h.vocab - first : plan.piece;
     const ProbEpilogue<T> pe{h.target, lse, f.d, h.tokens, rows, first, plan.d, plan.piece};
     rc = launch_product<T, false, false>(logits_problem(h, first, rows),
-                                         cut_for(rows, h.tokens, steps_of(h.hidden * 2), false), pe,
+                                         cut_for(rows, h.tokens, steps_of(h.hidden * 2), kNoSlices), pe,
                                          s);
     if (rc) return rc;
     if (dx) {
@@ -712,7 +712,7 @@ int backward(const Head& h, int reduction, const float* lse, const float* count,
       pw.k_bytes = (int)(up_to(h.tokens, 8) * 2);
       const WeightGradEpilogue<T> we{dw + first * h.hidden, rows, h.hidden, f.dw};
       rc = launch_product<T, true, true>(
-          pw, cut_for(h.hidden, rows, steps_of(pw.k_bytes), false), we, s);
+          pw, cut_for(h.hidden, rows, steps_of(pw.k_bytes), kNoSlices), we, s);
       if (rc) return rc;
     }
   }

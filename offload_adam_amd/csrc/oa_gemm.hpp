@@ -193,19 +193,17 @@ __device__ __forceinline__ i32x4 tile_rsrc(const Operand& o, int64_t row0, int t
   return descriptor(o.base + (rows > 0 ? row0 * o.ld : 0) + k, (int)(rows * o.ld));
 }
 
-// Slice and tile of workgroup b of `total`: consecutive workgroups go to the 8 XCDs in
-// turn, and each XCD gets one contiguous run of numbers, slices outermost and tiles so that
-// a run covers blocks of kGroup tiles along p: the operands of the tiles that an XCD has in
-// flight together then come out of its own L2.
+// Consecutive workgroups go to the 8 XCDs in turn; each XCD gets one contiguous run of
+// numbers, so that neighbours share an L2.
+__device__ __forceinline__ uint32_t in_runs(uint32_t b, uint32_t total) {
+  const uint32_t per = total / kXcds, extra = total % kXcds, x = b % kXcds;
+  return x * per + (x < extra ? x : extra) + b / kXcds;
+}
+// Tiles are numbered in blocks of kGroup along p: the operands of the tiles that an XCD has
+// in flight together then come out of its own L2.
 constexpr int kGroup = 8;
-__device__ __forceinline__ void tile_of(uint32_t b, uint32_t total, uint32_t tiles_p,
-                                        uint32_t tiles_q, uint32_t& slice, uint32_t& tp,
-                                        uint32_t& tq) {
-  const uint32_t per = total / kXcds, extra = total % kXcds;
-  const uint32_t x = b % kXcds, j = b / kXcds;
-  uint32_t id = x * per + (x < extra ? x : extra) + j;
-  slice = id / (tiles_p * tiles_q);
-  id -= slice * tiles_p * tiles_q;
+__host__ __device__ __forceinline__ void tile_at(uint32_t id, uint32_t tiles_p, uint32_t tiles_q,
+                                                 uint32_t& tp, uint32_t& tq) {
   const uint32_t group = id / (kGroup * tiles_q);
   const uint32_t first = group * kGroup;
   const uint32_t wide = tiles_p - first < kGroup ? tiles_p - first : kGroup;
@@ -746,14 +744,21 @@ struct Tile {
   }
 };
 
-// One product.  `slices` workgroups share a tile, each with its own run of k steps;
-// what becomes of their results is the epilogue's business.
+// One product.  The first `whole` tiles have a workgroup each; the others are cut along k
+// and have `slices`, each with its own run of steps; what becomes of their results is the
+// epilogue's business.
 struct Problem {
   Operand q, p;
   Scales sq, sp;  // e4m3 only
   int k_bytes;
   int steps_per_slice;
-  uint32_t tiles_q, tiles_p;
+  uint32_t tiles_q, tiles_p, whole;
+};
+// What a workgroup has: column tq of the tiles, and of a cut tile the slice and the tile's
+// number among those; slice -1: a whole tile.
+struct Place {
+  int tq, slice;
+  uint32_t number;
 };
 
 inline int steps_of(int64_t k_bytes) { return (int)((k_bytes + kStepBytes - 1) / kStepBytes); }
@@ -762,14 +767,28 @@ template <class T, class E>
 __global__ void __launch_bounds__(T::kThreads) product_kernel(const Problem pr, const E epilogue) {
   __shared__ __align__(16) uint8_t lds[T::kLdsBytes];
   T t;
-  uint32_t slice, tp, tq;
-  tile_of(blockIdx.x, gridDim.x, pr.tiles_p, pr.tiles_q, slice, tp, tq);
-  const int64_t row_q = (int64_t)tq * T::BQ, row_p = (int64_t)tp * T::BP;
   const int steps = (pr.k_bytes + kStepBytes - 1) / kStepBytes;
-  const int step0 = (int)slice * pr.steps_per_slice;
-  const int step1 = step0 + pr.steps_per_slice < steps ? step0 + pr.steps_per_slice : steps;
+  int step0 = 0, step1 = steps;
+  Place at{0, -1, 0};
+  uint32_t id;
+  if (blockIdx.x < pr.whole) {
+    id = in_runs(blockIdx.x, pr.whole);
+  } else {
+    // slices outermost: an XCD works on tiles of one slice
+    const uint32_t cut = pr.tiles_p * pr.tiles_q - pr.whole;
+    const uint32_t v = in_runs(blockIdx.x - pr.whole, gridDim.x - pr.whole);
+    at.slice = (int)(v / cut);
+    at.number = v - (uint32_t)at.slice * cut;
+    id = pr.whole + at.number;
+    step0 = at.slice * pr.steps_per_slice;
+    if (step0 + pr.steps_per_slice < steps) step1 = step0 + pr.steps_per_slice;
+  }
+  uint32_t tp, tq;
+  tile_at(id, pr.tiles_p, pr.tiles_q, tp, tq);
+  at.tq = (int)tq;
+  const int64_t row_q = (int64_t)tq * T::BQ, row_p = (int64_t)tp * T::BP;
   t.run(pr.q, pr.p, row_q, row_p, pr.k_bytes, step0, step1, pr.sq, pr.sp, lds);
-  epilogue(t, row_q, row_p, (int)tq, (int)slice, lds);
+  epilogue(t, row_q, row_p, at, lds);
 }
 
 // Tile sizes: 256 x 256, one workgroup to a CU, and 128 x 128, two to a CU.  A step of
@@ -783,11 +802,14 @@ using Small = Tile<T, 128, KQ, KP>;
 
 inline int64_t tiles_along(int64_t rows, int64_t tile) { return (rows + tile - 1) / tile; }
 
-// How a product is cut: into which tiles, and each tile along k into how many slices.
+// How a product is cut: into which tiles, and into how many slices along k those from
+// number `whole` on.
 struct Cut {
   bool large;
   int slices;
+  int64_t whole;
 };
+enum Slicing { kNoSlices, kAllTiles, kLastTiles };  // what may be cut
 
 // The cut with the least estimated time, in microseconds.  A round of n workgroups takes
 // steps times the time of a step, plus what a tile costs besides.  The time of a step grows
@@ -797,28 +819,34 @@ struct Cut {
 // e4m3, 4096 x 5632 x 2048: 52 us small, 58 large; 4096 x 14336 x 4096: 209 large, 248
 // small; bf16, 4096 x 2048 x 16384: 190 large in two slices, 260 small; 484 x 232 x 37632:
 // 29 small in 12 slices, 40 in 49.
-inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, bool may_slice) {
-  Cut best{false, 1};
+// kLastTiles: the tiles of a round that is not full are cut even behind full ones: e4m3, dx
+// and dw of 10395 tokens, 2176 -> 11600 (1.4 and 1.6 rounds): 610 us, 541 so; 4300 x 4096 x
+// 4096 (1.06 rounds), 89 and 85.  Where power is the limit (16384 x 14336 x 4096, 3.5
+// rounds) it gains nothing and loses nothing.
+inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, Slicing slicing) {
+  Cut best{false, 1, 0};
   double least = 0.0;
   for (int large = 0; large < 2; ++large) {
     const int64_t side = large ? 256 : 128, room = large ? 256 : 512;
     const double base = large ? 0.95 : 0.42, more = large ? 0.55 : 0.53;
     const double besides = large ? 7.0 : 3.0;
     const int64_t tiles = tiles_along(rows_q, side) * tiles_along(rows_p, side);
-    int64_t most = may_slice ? room / tiles : 1;  // a full chip is not cut further
+    const int64_t whole = tiles / room * room, rest = tiles - whole;
+    int64_t most = 1;  // a full chip is not cut further
+    if (rest && (slicing == kLastTiles || (slicing == kAllTiles && !whole))) most = room / rest;
     if (most > steps / 4) most = steps / 4;
     if (most < 1) most = 1;
     for (int64_t slices = 1; slices <= most; ++slices) {
-      const int64_t n = tiles * slices, rest = n % room;
-      const double s = (double)tiles_along(steps, slices);
-      double t = (double)(n / room) * (s * (base + more) + besides);
-      if (rest) t += s * (base + more * (double)rest / (double)room) + besides;
+      double t = (double)(whole / room) * (steps * (base + more) + besides);
+      const double n = (double)(rest * slices) / (double)room;
+      if (rest) t += (double)tiles_along(steps, slices) * (base + more * n) + besides;
       if (slices > 1)
         t += 3.0 + 0.1 * (double)slices +
-             (double)rows_q * (double)rows_p * 8.0 * (double)slices / 4e6;
+             (double)rows_q * (double)rows_p * (double)rest / (double)tiles * 8.0 *
+                 (double)slices / 4e6;
       if (least == 0.0 || t < least) {
         least = t;
-        best = Cut{large != 0, (int)slices};
+        best = Cut{large != 0, (int)slices, slices > 1 ? whole : 0};
       }
     }
   }
@@ -826,22 +854,24 @@ inline Cut cut_for(int64_t rows_q, int64_t rows_p, int steps, bool may_slice) {
 }
 
 template <class T, class E>
-int launch_tiles(Problem pr, int slices, const E& epilogue, hipStream_t stream) {
+int launch_tiles(Problem pr, const Cut& cut, const E& epilogue, hipStream_t stream) {
   const int64_t tq = tiles_along(pr.q.rows, T::BQ), tp = tiles_along(pr.p.rows, T::BP);
-  if (tq * tp * slices > 0x7FFFFFFF) return OA_ERANGE;
+  const int64_t workgroups = cut.whole + (tq * tp - cut.whole) * cut.slices;
+  if (workgroups > 0x7FFFFFFF) return OA_ERANGE;
   pr.tiles_q = (uint32_t)tq;
   pr.tiles_p = (uint32_t)tp;
+  pr.whole = (uint32_t)cut.whole;
   const int steps = steps_of(pr.k_bytes);
-  pr.steps_per_slice = (steps + slices - 1) / slices;
-  hipLaunchKernelGGL((product_kernel<T, E>), dim3((unsigned)(tq * tp * slices)),
-                     dim3(T::kThreads), 0, stream, pr, epilogue);
+  pr.steps_per_slice = (steps + cut.slices - 1) / cut.slices;
+  hipLaunchKernelGGL((product_kernel<T, E>), dim3((unsigned)workgroups), dim3(T::kThreads), 0,
+                     stream, pr, epilogue);
   return launch_status();
 }
 
 template <class T, bool KQ, bool KP, class E>
 int launch_product(const Problem& pr, const Cut& cut, const E& epilogue, hipStream_t stream) {
-  return cut.large ? launch_tiles<Large<T, KQ, KP>, E>(pr, cut.slices, epilogue, stream)
-                   : launch_tiles<Small<T, KQ, KP>, E>(pr, cut.slices, epilogue, stream);
+  return cut.large ? launch_tiles<Large<T, KQ, KP>, E>(pr, cut, epilogue, stream)
+                   : launch_tiles<Small<T, KQ, KP>, E>(pr, cut, epilogue, stream);
 }
 
 // Carves a workspace; with a null base it only counts.

@@ -200,14 +200,16 @@ def test_the_bias_gradient_is_the_plain_sum():
            gy[:, keep].double(), "db", codes=False)
 
 
-@pytest.mark.parametrize("shape", [(4096, 512, 3200), (3000, 2048, 4000)])
+@pytest.mark.parametrize("shape", [(4096, 512, 3200), (3000, 2048, 4000), (4300, 4096, 4001),
+                                   (4000, 4304, 4096), (2300, 8000, 4100)])
 def test_large_tiles(shape):
+    """The last three: more tiles than CUs, those that are over cut along k."""
     t, k, n = shape
-    x, q, _, gy = _layer(t, k, n, BF16, seed=4)
-    y = F.linear(x, q)
+    x, q, b, gy = _layer(t, k, n, BF16, seed=4, bias=True)
+    y = F.linear(x, q, b)
     dx, dw = torch.autograd.grad(y, (x, q), gy)
     xv, w = x.detach(), q.detach().dequantize(F32).double()
-    _close(y.detach(), _held(xv, 1), w.t(), "y")
+    _close(y.detach(), _held(xv, 1), w.t(), "y", b.detach().double())
     _close(dx, _held(gy, 1), w, "dx")
     _close(dw, _held(gy, 0).t(), _held(xv, 0), "dw")
 
