@@ -22,6 +22,8 @@ def _rows(t, name):
     """2-D operand of the kernels: unit column stride, columns and row stride multiples
     of 8 elements, 16-byte aligned.  Anything else is copied, zero-padded."""
     rows, cols = t.shape
+    if cols % 8 == 0 and cols <= 1 << 20 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, cols, cols
     stride = t.stride(0) if rows > 1 else -(-cols // 8) * 8
     if (cols % 8 == 0 and (cols == 1 or t.stride(1) == 1) and stride >= cols and stride % 8 == 0
             and stride <= 1 << 20 and t.data_ptr() % 16 == 0):
@@ -143,6 +145,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
         raise ValueError("x must be a GPU tensor (no CPU path exists)")
     if weight.device != x.device or target.device != x.device:
         raise ValueError("x, weight and target must be on the same GPU")
-    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight,
-                                     target.reshape(-1).contiguous(), int(ignore_index), reduction)
+    flat, rows = target, x
+    if target.dim() != 1:
+        flat, rows = target.reshape(-1), x.reshape(-1, x.shape[-1])
+    loss = _LinearCrossEntropy.apply(rows, weight, flat.contiguous(), int(ignore_index), reduction)
     return loss.reshape(target.shape) if reduction == "none" else loss

@@ -102,8 +102,12 @@ def _quantize_fp8_hip(tensor):
     return weight, scale
 
 
+def _rows_of(x):
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
 def _linear_forward(x, weight, bias):
-    flat = x.reshape(-1, x.shape[-1])
+    flat = _rows_of(x)
     if x.is_cuda:
         y = _codec_ops.fp8_linear_forward(flat, weight.weight, weight.block_scale, bias)
     else:
@@ -126,8 +130,7 @@ class _FP8Linear(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight = ctx.saved_tensors
         want_dx, want_dw, want_db = ctx.needs_input_grad
-        flat = x.reshape(-1, x.shape[-1])
-        g = grad.reshape(-1, weight.weight.shape[0])
+        flat, g = _rows_of(x), _rows_of(grad)
         if x.is_cuda:
             dx, dw, db = _codec_ops.fp8_linear_backward(
                 g, flat, weight.weight, weight.block_scale, want_dx, want_dw, want_db)
@@ -139,7 +142,9 @@ class _FP8Linear(torch.autograd.Function):
                 dw = (_held(g, FP8_BLOCK, 1).T @ _held(flat, FP8_BLOCK, 1)).to(x.dtype)
             if want_db:
                 db = g.float().sum(0).to(x.dtype)
-        return dx.reshape(x.shape) if want_dx else None, dw, db
+        if want_dx and x.dim() != 2:
+            dx = dx.reshape(x.shape)
+        return dx, dw, db
 
 
 class FP8QWeight(QWeightBase):
