@@ -534,8 +534,8 @@ struct CutEpilogue {
 
 // ---- few tokens.  Bound by reading the weight once.  A workgroup makes 16 columns of y;
 // each of its waves takes every WAVES-th step of k, its fragments straight from memory to
-// registers (16 rows of 128 bytes each), two or four steps ahead of the products, so that the
-// loads of all waves of a CU cover the latency, multiplies them with all the tokens, one or
+// registers (16 rows of 128 bytes each), two or four steps ahead of the products, so that
+// the loads of all waves of a CU cover the latency, multiplies them with all the tokens, one or
 // two tiles of 16, and the waves' sums meet in LDS, in order.  ENCODE: x comes as it is
 // and every workgroup makes the codes for itself, in LDS, while its weights are on the way.
 template <int DT>
@@ -558,7 +558,7 @@ template <int DT, int TILES, int WAVES, bool ENCODE>
 __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) {
   static_assert(!ENCODE || TILES == 1, "a workgroup encodes the tokens of one tile");
   constexpr int kLanes = WAVES * kWave;
-  constexpr int kFewAhead = TILES * WAVES >= 32 ? 2 : 4;  // what the registers hold
+  constexpr int kFewAhead = ENCODE ? 4 : 2;  // codes of x on their way take registers too
   constexpr int kPieces = ENCODE ? kFewCodes / kPatch / kLanes : 1;
   __shared__ __align__(16) float sums[WAVES][TILES][kLines][kLines + 4];  // [token][column]
   __shared__ __align__(16) uint8_t codes[ENCODE ? kFewCodes : 16];
@@ -569,9 +569,20 @@ __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t n0 = (int64_t)blockIdx.x * kLines;
   const int r = lane % kLines, k0 = lane / kLines * 32;
-  const int64_t n = n0 + r < a.out_f ? n0 + r : a.out_f - 1;  // rows past the end: not stored
-  const uint8_t* wrow = a.w + n * a.in_f + k0;
-  const uint8_t* scale = a.ws + n0 / kBlock * a.blocks_k;
+  // What is not there reads as zero by the descriptors' ranges, without a branch: behind one
+  // the compiler does not know how many loads are on their way, and waits for all.
+  const int rows = a.out_f - n0 < kLines ? (int)(a.out_f - n0) : kLines;
+  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w + n0 * a.in_f), 0, rows * a.in_f, 0x00020000);
+  const auto ws_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.ws + n0 / kBlock * a.blocks_k), 0, a.blocks_k, 0x00020000);
+  const auto xq_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.xq), 0, a.tokens * (int)a.ldx, 0x00020000);
+  const auto xs_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.xs), 0, a.blocks_k * (int)a.xs_stride, 0x00020000);
+  auto load16 = [](auto rsrc, int at) {
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+  };
   f32x4 acc[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -590,27 +601,20 @@ __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) 
   }
   auto fetch = [&](int step, i32x8& q, int& sq, i32x8 (&p)[TILES], int (&sp)[TILES]) {
     const int k = step * kStepBytes + k0;
-    i32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    sq = 0;
-    if (step < a.blocks_k) {
-      if (k < a.in_f) lo = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes);
-      if (k + 16 < a.in_f) hi = *reinterpret_cast<const i32x4*>(wrow + step * kStepBytes + 16);
-      sq = scale[step];
-    }
+    const i32x4 lo = load16(w_rsrc, k < a.in_f ? r * a.in_f + k : kOut);
+    const i32x4 hi = load16(w_rsrc, k + 16 < a.in_f ? r * a.in_f + k + 16 : kOut);
     q = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    sq = __builtin_amdgcn_raw_buffer_load_b8(ws_rsrc, step, 0, 0);
     if constexpr (!ENCODE) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         const int token = t * kLines + r;
-        p[t] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-        sp[t] = 0;
-        if (step < a.blocks_k && token < a.tokens) {  // rows of codes are whole steps long
-          const uint8_t* at = a.xq + token * a.ldx + k;
-          p[t] = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(at),
-                                         *reinterpret_cast<const i32x4*>(at + 16), 0, 1, 2, 3, 4,
-                                         5, 6, 7);
-          sp[t] = a.xs[packed_scale_at(token, step, a.xs_stride)];
-        }
+        const bool in = step < a.blocks_k && token < a.tokens;  // rows are whole steps long
+        const int at = in ? token * (int)a.ldx + k : kOut;
+        p[t] = __builtin_shufflevector(load16(xq_rsrc, at), load16(xq_rsrc, at + 16), 0, 1, 2, 3,
+                                       4, 5, 6, 7);
+        sp[t] = __builtin_amdgcn_raw_buffer_load_b8(
+            xs_rsrc, in ? (int)packed_scale_at(token, step, a.xs_stride) : kOut, 0, 0);
       }
     }
   };
@@ -643,23 +647,24 @@ __global__ void __launch_bounds__(WAVES* kWave) fp8_few_kernel(const Few<DT> a) 
 #pragma unroll
     for (int i = 0; i < kFewAhead; ++i) {
       const int at = step + i * WAVES;
-      if (at < a.blocks_k) {
-        if constexpr (ENCODE) {
-          p[i][0] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
-          sp[i][0] = 0;
-          if (r < a.tokens) {
-            const uint8_t* c = codes + r * (int)a.ldx + at * kStepBytes + k0;
-            p[i][0] = __builtin_shufflevector(*reinterpret_cast<const i32x4*>(c),
-                                              *reinterpret_cast<const i32x4*>(c + 16), 0, 1, 2, 3,
-                                              4, 5, 6, 7);
-            sp[i][0] = scales[r * a.blocks_k + at];
-          }
-        }
+      if constexpr (ENCODE) {
+        const bool in = at < a.blocks_k && r < a.tokens;
+        const uint8_t* c = codes + (in ? r * (int)a.ldx + at * kStepBytes + k0 : 0);
+        const i32x4 lo = *reinterpret_cast<const i32x4*>(c);
+        const i32x4 hi = *reinterpret_cast<const i32x4*>(c + 16);
+        const int s = scales[in ? r * a.blocks_k + at : 0];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[i], p[i][t], acc[t], 0, 0, 0,
-                                                                    sq[i], 0, sp[i][t]);
+        for (int j = 0; j < 4; ++j) {
+          p[i][0][j] = in ? lo[j] : 0;
+          p[i][0][4 + j] = in ? hi[j] : 0;
+        }
+        sp[i][0] = in ? s : 0;
       }
+      // steps past the last: zeros
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+        acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[i], p[i][t], acc[t], 0, 0, 0,
+                                                                  sq[i], 0, sp[i][t]);
       fetch(at + kFewAhead * WAVES, q[i], sq[i], p[i], sp[i]);
     }
   }
@@ -687,7 +692,7 @@ void launch_few(const Few<DT>& a, int waves, hipStream_t s) {
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 4, ENCODE>), grid, block, 0, s, a);
   else if (waves == 8)
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 8, ENCODE>), grid, block, 0, s, a);
-  else
+  else if constexpr (ENCODE)
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 16, ENCODE>), grid, block, 0, s, a);
 }
 
@@ -796,18 +801,19 @@ struct Layer {
 
 // Whether the kernel for few tokens takes a call.  It reads every token's codes once per 16
 // columns, the tiles once per 128, but those take two more launches and half the bytes they
-// move in LDS are for rows that hold no token.  4096 -> 14336: 15, 17 and 24 us for 1, 4 and
+// move in LDS are for rows that hold no token.  4096 -> 14336: 15, 17 and 23 us for 1, 4 and
 // 16 tokens, 22 with tiles; 28 against 22 for 24; a small weight gains for longer: 4096 ->
-// 4096, 24 tokens, 11 against 15, 64 tokens 16 and 16.
+// 4096, 24 tokens, 11 against 15.
 bool takes_few(const Layer& w, int64_t tokens) {
   return tokens <= kLines || (tokens <= 2 * kLines && w.out_f * w.in_f <= (1 << 24));
 }
 // Waves of its workgroups: a CU that has only one of them needs more loads in flight from
-// it.  1 token, 4 / 8 / 16 waves: 4096 -> 14336, 15.4, 16.1, 19.5 us; 14336 -> 4096, 22.3,
-// 15.8, 13.5; 4096 -> 4096, 8.0, 6.4, 6.3; 2048 -> 5632, 5.6, 6.0, 7.6.
-int few_waves(const Layer& w) {
+// it.  1 token, 4 / 8 / 16 waves: 4096 -> 14336, 14.6, 14.1, 19.6 us; 2048 -> 5632, 5.3, 6.0,
+// 8.6; 4096 -> 4096, 6.1, 5.7, 6.2; 14336 -> 4096, 13.8, 13.5, 12.9.  8 tokens: 4096 ->
+// 14336, 20.8, 21.1, 25.2; 14336 -> 4096, 21.5, 18.3, 19.3.
+int few_waves(const Layer& w, bool encode) {
   if (tiles_along(w.out_f, kLines) > 256) return 4;
-  return blocks_of(w.in_f) < 64 ? 8 : 16;
+  return encode && blocks_of(w.in_f) >= 64 ? 16 : 8;
 }
 
 struct ForwardPlan {
@@ -830,11 +836,13 @@ int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws
   const bool few = takes_few(w, x.rows);
   const ForwardPlan plan(x.rows, w.in_f, w.out_f, few, ws);
   if (few) {
-    const int waves = few_waves(w), tokens = (int)x.rows;
+    const int tokens = (int)x.rows;
+    const bool encode = tokens <= kFewEncodeTokens && tokens * plan.x.ld <= kFewCodes;
+    const int waves = few_waves(w, encode);
     const Few<DT> a{w.q, w.scales, w.out_f, (int)w.in_f, (int)blocks_of(w.in_f),
                     x, plan.x.q, plan.x.scales, plan.x.ld,
                     plan.x.scale_stride, tokens, bias, y};
-    if (tokens <= kFewEncodeTokens && tokens * plan.x.ld <= kFewCodes) {
+    if (encode) {
       launch_few<DT, 1, true>(a, waves, s);
       return launch_status();
     }
