@@ -213,13 +213,24 @@ class FP8QWeight(QWeightBase):
     @classmethod
     def from_plain_state_dict(cls, plain: dict, reference=None) -> "FP8QWeight":
         """Scales that are powers of two are taken as they are; a checkpoint with any
-        other (finite, positive) scales is encoded again from the values it stands for."""
+        other (finite, not negative) scales is encoded again from the values it stands for.
+        Other block sizes than 128 x 128 are refused."""
         if reference is None:
             raise ValueError(
                 "FP8QWeight.from_plain_state_dict requires a reference instance to "
                 "resolve outer_dtype; the canonical state_dict carries no outer-dtype field."
             )
         weight, scale = plain["weight"], plain["weight_scale_inv"].float()
+        if weight.dtype is not torch.float8_e4m3fn or weight.dim() != 2 or weight.shape[1] % 16:
+            raise ValueError(f"weight must be a float8_e4m3fn matrix with a multiple of 16 columns, "
+                             f"got {weight.dtype} {tuple(weight.shape)}")
+        grid = tuple(-(-n // FP8_BLOCK) for n in weight.shape)
+        if tuple(scale.shape) != grid:
+            raise ValueError(
+                f"weight_scale_inv of a {tuple(weight.shape)} weight must have shape {grid} (blocks "
+                f"of {FP8_BLOCK} x {FP8_BLOCK}), got {tuple(scale.shape)}")
+        if not bool(((scale >= 0) & torch.isfinite(scale)).all()):
+            raise ValueError("weight_scale_inv must be finite and not negative")
         bits = scale.view(torch.int32)
         exponent = bits >> 23  # sign and exponent field of a positive normal number
         if bool(((bits & 0x7FFFFF) == 0).all() and ((exponent > 0) & (exponent < 255)).all()):

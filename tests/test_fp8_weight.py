@@ -145,6 +145,44 @@ def test_checkpoints_with_other_scales_are_encoded_again():
         FP8QWeight.from_plain_state_dict({"weight": codes, "weight_scale_inv": scale})
 
 
+@pytest.mark.parametrize("power", [False, True])
+def test_checkpoints_that_do_not_fit_are_refused(power):
+    """Scales of finer, coarser or transposed blocks, or that are no scales; codes of another
+    type or of an odd width.  A weight of another shape is torch's own size mismatch."""
+    g = torch.Generator().manual_seed(4)
+    model = nn.Sequential(nn.Linear(256, 384, bias=False)).to(BF16)
+    quantize_linears(model, FP8QWeight)
+    before = model[0].weight.data.dequantize()
+    codes = torch.randn(384, 256, generator=g).mul(50).to(torch.float8_e4m3fn)
+
+    def scales(*grid):
+        return torch.full(grid, 0.5) if power else torch.rand(grid, generator=g) + 0.3
+
+    def load(weight, scale):
+        return model.load_state_dict({"0.weight": weight, "0.weight_scale_inv": scale})
+
+    for grid in ((6, 4), (1, 1), (2, 3), (3, 1), (6,), ()):
+        with pytest.raises(ValueError, match="weight_scale_inv"):
+            load(codes, scales(*grid))
+    for bad in (float("nan"), float("inf"), -1.0):
+        scale = scales(3, 2)
+        scale[1, 1] = bad
+        with pytest.raises(ValueError, match="weight_scale_inv"):
+            load(codes, scale)
+    for weight in (codes.view(torch.uint8), codes.to(torch.float8_e5m2), codes[:, :250], codes[0]):
+        with pytest.raises(ValueError, match="weight must be"):
+            FP8QWeight.from_plain_state_dict({"weight": weight, "weight_scale_inv": scales(3, 2)},
+                                             model[0].weight.data)
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        load(codes[:256], scales(2, 2))
+    assert torch.equal(model[0].weight.data.dequantize(), before)
+    # a block of zeros may come with a scale of zero
+    scale = scales(3, 2)
+    scale[0, 0] = 0.0
+    load(codes, scale)
+    assert not model[0].weight.data.dequantize()[:128, :128].any()
+
+
 def test_refused_arguments():
     w = FP8QWeight.from_float(torch.randn(32, 64))
     x = torch.randn(4, 64)
