@@ -32,6 +32,7 @@ from typing import Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _codec_ops
@@ -249,6 +250,10 @@ class FP8QWeight(QWeightBase):
         }
 
 
+def _tangent(t):
+    return t is not None and forward_ad.unpack_dual(t).tangent is not None
+
+
 @FP8QWeight.implements_torch_function(torch.nn.functional.linear)
 def _linear(func, types, args, kwargs):
     def run(input, weight, bias=None):
@@ -267,9 +272,10 @@ def _linear(func, types, args, kwargs):
                 raise ValueError(f"linear: bias must have shape ({codes.shape[0]},) on "
                                  f"{input.device}, got {tuple(bias.shape)} on {bias.device}")
             bias = bias.to(input.dtype).contiguous()
-        if not torch.is_grad_enabled() or not (
+        # also for tangents, which the function refuses: the kernels would drop them
+        if not (_tangent(input) or _tangent(bias)) and (not torch.is_grad_enabled() or not (
                 input.requires_grad or weight.requires_grad
-                or (bias is not None and bias.requires_grad)):
+                or (bias is not None and bias.requires_grad))):
             return _linear_forward(input, weight, bias)
         return _FP8Linear.apply(input, weight, bias)
 

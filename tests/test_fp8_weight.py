@@ -8,6 +8,7 @@ import pytest
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from offload_adam_amd import _lib
 from offload_adam_amd.qweight import FORMATS, FP8QWeight, quantize_linears
@@ -96,6 +97,25 @@ def test_linear_and_its_gradients():
     assert (dx.reshape(-1, 144).double() - held(gy, 1, 128) @ wv).abs().max() < 210 * 2**-23 * 600
     assert (dw.double() - held(gy, 128, 1).T @ held(flat, 128, 1)).abs().max() < 210 * 2**-23 * 600
     assert (db.double() - gy.double().sum(0)).abs().max() < 210 * 2**-23 * 210
+
+
+def test_forward_mode_is_refused():
+    """A layer that nothing requires a gradient of has no tangents either, as the other
+    formats' layers."""
+    w = FP8QWeight.from_float(torch.randn(32, 64))
+    x, b = torch.randn(4, 64), torch.randn(32)
+    plain = F.linear(x, w, b)
+    with forward_ad.dual_level():
+        assert torch.equal(F.linear(x, w, b), plain)
+        for args in ((forward_ad.make_dual(x, torch.ones_like(x)), w, b),
+                     (x, w, forward_ad.make_dual(b, torch.ones_like(b)))):
+            with pytest.raises(NotImplementedError):
+                F.linear(*args)
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                F.linear(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: F.linear(t, w), (x,), (torch.ones_like(x),))
+    assert torch.equal(F.linear(x, w, b), plain)
 
 
 def test_state_dict_and_config(tmp_path):
