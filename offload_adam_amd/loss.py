@@ -10,7 +10,6 @@ gradients.  The reference has no counterpart: its example's model returns logits
 """
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .qweight import base as _qbase
@@ -75,7 +74,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_qbase.first_derivatives_only
     def backward(ctx, grad):
         x, weight, target, stats = ctx.saved_tensors
         want_dx, want_dw = ctx.needs_input_grad[:2]
@@ -117,8 +116,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     ``"sum"``, or ``"none"`` (losses of ``target``'s shape).  The loss is fp32;
     logits, exponentials and sums are fp32 throughout, and only the logits' gradient is
     rounded to 16 bits, once, between the two products that use it.  Gradients flow to
-    ``x`` and ``weight``; second derivatives are not available.  Results do not depend
-    on anything but the arguments: no atomics, one order of summation.
+    ``x`` and ``weight``; taking second derivatives or forward-mode ones raises.  Results
+    do not depend on anything but the arguments: no atomics, one order of summation.
 
     Works on ``x``'s device and the current stream, synchronises nothing, and may be
     captured into a graph, with the backward pass inside the same capture and no eager

@@ -18,6 +18,8 @@ every format shares are registered once, for each subclass, from
 dequantise routines and how a dtype change maps onto its payload.
 """
 
+import functools
+
 import torch
 from torch import Tensor
 from torch.utils._python_dispatch import return_and_correct_aliasing
@@ -53,6 +55,35 @@ def _dequantized(weight, dtype):
     w = weight.dequantize(dtype=dtype)
     weight.__dict__["_dequantized_cache"] = (key, w)
     return w
+
+
+class _Refusal(torch.autograd.Function):
+    """The first ``count`` tensors, on which differentiating by any of the others fails."""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(None if t is None else t.clone() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("second derivatives of this operator are not available")
+
+
+def first_derivatives_only(backward):
+    """Decorator of a function's ``backward`` that is not differentiable.  With
+    ``create_graph`` its results hang on everything they were computed from, so that a
+    second derivative raises; ``once_differentiable`` lets it be zero where the incoming
+    gradient is a constant or is what it is taken by."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _Refusal.apply(len(out), *out, *grads, *ctx.saved_tensors)
+
+    return wrapper
 
 
 class _WeightOnlyLinear(torch.autograd.Function):

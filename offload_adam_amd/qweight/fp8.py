@@ -24,8 +24,9 @@ activations' dtype, ``F.linear`` on this one also encodes its other operand, in 
 with fp32 sums and one rounding to the dtype of ``x``.  (The matrix instruction adds the
 products of eight neighbouring elements with their 13 highest bits, counted from the largest
 of the eight, before they enter the fp32 sum: an error of up to 7 * 2^-13 of that product,
-where the codes themselves are off by 2^-4 each.)  The reference has no counterpart (its
-formats are weight-only, src/offload_adam/qweight/).
+where the codes themselves are off by 2^-4 each.)  Taking second derivatives or
+forward-mode ones raises.  The reference has no counterpart (its formats are weight-only,
+src/offload_adam/qweight/).
 """
 
 from typing import Tuple
@@ -33,10 +34,9 @@ from typing import Tuple
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import _codec_ops
-from .base import QWeightBase
+from .base import QWeightBase, first_derivatives_only
 
 FP8_BLOCK = _codec_ops.FP8_BLOCK
 FP8_E4M3_MAX = 448.0
@@ -127,7 +127,7 @@ class _FP8Linear(torch.autograd.Function):
         return _linear_forward(x, weight, bias)
 
     @staticmethod
-    @once_differentiable
+    @first_derivatives_only
     def backward(ctx, grad):
         x, weight = ctx.saved_tensors
         want_dx, want_dw, want_db = ctx.needs_input_grad

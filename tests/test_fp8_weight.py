@@ -118,6 +118,28 @@ def test_forward_mode_is_refused():
     assert torch.equal(F.linear(x, w, b), plain)
 
 
+def test_second_derivatives_are_refused():
+    """Also where the incoming gradient is a constant, and where a tangent is taken by
+    differentiating twice: neither may come out as zero."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(4, 64, generator=g).requires_grad_(True)
+    w = nn.Parameter(FP8QWeight.from_float(torch.randn(32, 64, generator=g)))
+    b = torch.randn(32, generator=g).requires_grad_(True)
+    up = torch.randn(4, 32, generator=g)
+    want = torch.autograd.grad(F.linear(x, w, b), (x, w, b), up)
+    got = torch.autograd.grad(F.linear(x, w, b), (x, w, b), up, create_graph=True)
+    assert all(torch.equal(i, j) for i, j in zip(want, got))
+    y = F.linear(x, w, b).sum()
+    dx, dw = torch.autograd.grad(y, (x, w), create_graph=True)
+    for penalty, by in ((dx, w), (dw, x), (y + dx.square().sum(), x)):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(penalty.sum(), by, retain_graph=True, allow_unused=True)
+    for leaves in ((x, w, b), (x, w.detach(), None)):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.functional.jvp(lambda t: F.linear(t, *leaves[1:]), (x.detach(),),
+                                          (torch.ones_like(x),))
+
+
 def test_state_dict_and_config(tmp_path):
     from safetensors.torch import load_file, save_file
 

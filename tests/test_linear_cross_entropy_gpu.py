@@ -251,6 +251,24 @@ def test_one_gradient_at_a_time_gives_the_same_bits():
         assert not linear_cross_entropy(a, b, y).requires_grad
 
 
+def test_second_derivatives_are_refused():
+    from offload_adam_amd import linear_cross_entropy
+
+    x, w, y = _inputs(20, 64, 100, BF16)
+    one = torch.ones((), device="cuda")
+    want = _run(x, w, y, one)
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(x, w, y)
+    dx, dw = torch.autograd.grad(loss, (x, w), create_graph=True)
+    assert torch.equal(dx.detach(), want[1]) and torch.equal(dw.detach(), want[2])
+    for penalty, by in ((dx, w), (dw, x), (loss + dx.float().square().sum(), x)):
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(penalty.sum(), by, retain_graph=True, allow_unused=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.functional.jvp(lambda t: linear_cross_entropy(t, w, y), (x.detach(),),
+                                      (torch.ones_like(x),))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 def test_tokens_whose_gradient_is_zero(dtype, reduction):
