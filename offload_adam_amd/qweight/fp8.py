@@ -24,7 +24,8 @@ activations' dtype, ``F.linear`` on this one also encodes its other operand, in 
 with fp32 sums and one rounding to the dtype of ``x``.  (The matrix instruction adds the
 products of eight neighbouring elements with their 13 highest bits, counted from the largest
 of the eight, before they enter the fp32 sum: an error of up to 7 * 2^-13 of that product,
-where the codes themselves are off by 2^-4 each.)  Taking second derivatives or
+where the codes themselves are off by 2^-4 each.)  Under ``torch.autocast`` the input and
+the bias are cast to its dtype first, as a plain weight's are.  Taking second derivatives or
 forward-mode ones raises.  The reference has no counterpart (its formats are weight-only,
 src/offload_adam/qweight/).
 """
@@ -107,12 +108,17 @@ def _rows_of(x):
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
 
+def _product(a, b):
+    with torch.autocast("cpu", enabled=False):  # fp32 sums under it too
+        return a @ b
+
+
 def _linear_forward(x, weight, bias):
     flat = _rows_of(x)
     if x.is_cuda:
         y = _codec_ops.fp8_linear_forward(flat, weight.weight, weight.block_scale, bias)
     else:
-        y = _held(flat, 1, FP8_BLOCK) @ weight.dequantize(torch.float32).T
+        y = _product(_held(flat, 1, FP8_BLOCK), weight.dequantize(torch.float32).T)
         y = (y if bias is None else y + bias.float()).to(x.dtype)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[1])
 
@@ -138,9 +144,9 @@ class _FP8Linear(torch.autograd.Function):
         else:
             dx = dw = db = None
             if want_dx:
-                dx = (_held(g, 1, FP8_BLOCK) @ weight.dequantize(torch.float32)).to(x.dtype)
+                dx = _product(_held(g, 1, FP8_BLOCK), weight.dequantize(torch.float32)).to(x.dtype)
             if want_dw:
-                dw = (_held(g, FP8_BLOCK, 1).T @ _held(flat, FP8_BLOCK, 1)).to(x.dtype)
+                dw = _product(_held(g, FP8_BLOCK, 1).T, _held(flat, FP8_BLOCK, 1)).to(x.dtype)
             if want_db:
                 db = g.float().sum(0).to(x.dtype)
         if want_dx and x.dim() != 2:
@@ -267,6 +273,9 @@ def _linear(func, types, args, kwargs):
                              f"{tuple(codes.shape)} do not match")
         if input.device != codes.device:
             raise ValueError(f"linear: input is on {input.device}, weight on {codes.device}")
+        kind = input.device.type
+        if torch.is_autocast_enabled(kind):  # as for a plain weight
+            input = input.to(torch.get_autocast_dtype(kind))
         if bias is not None:
             if tuple(bias.shape) != (codes.shape[0],) or bias.device != input.device:
                 raise ValueError(f"linear: bias must have shape ({codes.shape[0]},) on "

@@ -140,6 +140,34 @@ def test_second_derivatives_are_refused():
                                           (torch.ones_like(x),))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, BF16])
+def test_autocast_casts_as_for_a_plain_weight(dtype):
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(5, 64, generator=g).to(dtype).requires_grad_(True)
+    plain = torch.randn(32, 64, generator=g)
+    w = nn.Parameter(FP8QWeight.from_float(plain))
+    b = torch.randn(32, generator=g).requires_grad_(True)
+    up = torch.randn(5, 32, generator=g).to(BF16)
+    with torch.autocast("cpu", dtype=BF16):
+        y = F.linear(x, w, b)
+        frozen = F.linear(x.detach(), w.detach(), b.detach())
+        assert F.linear(x.detach(), plain, b.detach()).dtype == y.dtype == frozen.dtype == BF16
+        inside = torch.autograd.grad(y, (x, w, b), up, retain_graph=True)
+    got = (y, *torch.autograd.grad(y, (x, w, b), up))
+    assert [v.dtype for v in got[1:]] == [dtype, torch.float32, torch.float32]
+    # the same as casting by hand: fp32 sums, one rounding
+    c, d = x.detach().to(BF16).requires_grad_(True), b.detach().to(BF16).requires_grad_(True)
+    want = F.linear(c, w, d)
+    want = (want, *torch.autograd.grad(want, (c, w, d), up))
+    assert torch.equal(frozen, want[0])
+    for i, j in zip(got, want):
+        assert torch.equal(i.float(), j.float())
+    for i, j in zip(got[1:], inside):
+        assert torch.equal(i, j)
+    with torch.autocast("cpu", dtype=BF16), pytest.raises(TypeError):
+        F.linear(x.detach().double(), w)
+
+
 def test_state_dict_and_config(tmp_path):
     from safetensors.torch import load_file, save_file
 

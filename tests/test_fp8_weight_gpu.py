@@ -273,6 +273,19 @@ def test_nothing_to_do():
     assert not dq.any() and not db.any()
 
 
+def test_autocast_casts_as_for_a_plain_weight():
+    x, q, b, gy = _layer(40, 144, 130, F32, bias=True)
+    for low in (BF16, F16):
+        c, d = x.detach().to(low).requires_grad_(True), b.detach().to(low).requires_grad_(True)
+        want = F.linear(c, q, d)
+        want = (want, *torch.autograd.grad(want, (c, q, d), gy.to(low)))
+        with torch.autocast("cuda", dtype=low):
+            y = F.linear(x, q, b)
+        got = (y, *torch.autograd.grad(y, (x, q, b), gy.to(low)))
+        assert y.dtype == low and all(v.dtype == F32 for v in got[1:])
+        assert all(torch.equal(i.float(), j.float()) for i, j in zip(got, want))
+
+
 def test_gradient_against_differences():
     """The layer is linear in its encoded input: steps that the codes hold exactly."""
     from offload_adam_amd.qweight import FP8QWeight
