@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from .qweight import base as _qbase
 
+_CASTABLE = (torch.float32, torch.float16, torch.bfloat16)
 _REDUCTIONS = {"none": _lib.OA_LOSS_NONE, "mean": _lib.OA_LOSS_MEAN, "sum": _lib.OA_LOSS_SUM}
 
 
@@ -108,7 +109,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
 
     ``x``: hidden states (..., hidden), bf16 or fp16, on the GPU; ``weight``: the output
     layer's (vocab, hidden) in the same dtype, or a quantised weight of this package
-    (decoded for the call); ``target``: int64 of ``x``'s leading shape.  Tokens whose
+    (decoded for the call); under ``torch.autocast`` both are cast to its dtype.
+    ``target``: int64 of ``x``'s leading shape.  Tokens whose
     target is ``ignore_index`` take no part: their losses and gradients are 0, whatever
     their rows of ``x`` hold.  Any other target outside [0, vocab) gives NaN.
 
@@ -126,11 +128,21 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     """
     if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
         raise TypeError("x and weight must be tensors")
+    decoded = weight.dtype
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    kind = x.device.type
+    if torch.is_autocast_enabled(kind):  # what F.linear casts
+        low = torch.get_autocast_dtype(kind)
+        if x.dtype in _CASTABLE:
+            x = x.to(low)
+        if weight.dtype in _CASTABLE:
+            decoded = low
+            if not isinstance(weight, _qbase.QWeightBase):
+                weight = weight.to(low)
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"x must be bfloat16 or float16, got {x.dtype}")
-    if weight.dtype != x.dtype:
+    if decoded != x.dtype:
         raise TypeError(f"weight must have x's dtype {x.dtype}, got {weight.dtype}")
     if not isinstance(target, torch.Tensor) or target.dtype != torch.int64:
         raise TypeError("target must be an int64 tensor")

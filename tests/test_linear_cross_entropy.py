@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from offload_adam_amd import _lib, linear_cross_entropy
+from offload_adam_amd.qweight import FP8QWeight
 
 BF16 = torch.bfloat16
 
@@ -35,6 +36,23 @@ def test_refused_arguments():
             linear_cross_entropy(*bad)
     with pytest.raises(ValueError, match="reduction"):
         linear_cross_entropy(x, w, y, reduction="average")
+
+
+def test_autocast_casts_before_the_checks():
+    x, w, y = _args(dtype=torch.float32)
+    for dtype in (BF16, torch.float16):
+        with torch.autocast("cpu", dtype=dtype):
+            for head in (w, w.to(BF16), FP8QWeight.from_float(w)):
+                with pytest.raises(ValueError, match="must be a GPU tensor"):  # only that is left
+                    linear_cross_entropy(x, head, y)
+            with pytest.raises(TypeError):
+                linear_cross_entropy(x.double(), w.double(), y)
+            with pytest.raises(TypeError):
+                linear_cross_entropy(x, w.double(), y)
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x, w, y)
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x.to(BF16), FP8QWeight.from_float(w), y)
 
 
 def test_the_c_entry_points_refuse_before_any_launch():

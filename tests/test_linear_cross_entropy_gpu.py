@@ -332,6 +332,27 @@ def test_quantised_head():
     assert all(torch.equal(i, j) for i, j in zip(got, want))
 
 
+@pytest.mark.parametrize("quantised", [False, True])
+def test_autocast_casts_as_for_plain_logits(quantised):
+    from offload_adam_amd import linear_cross_entropy
+    from offload_adam_amd.qweight import FP8QWeight
+
+    x, w, y = _inputs(70, 128, 300, BF16)
+    x = x.float().requires_grad_(True)
+    w = torch.nn.Parameter(FP8QWeight.from_float(w.float()) if quantised else w.float())
+    for low in (BF16, F16):
+        c = x.detach().to(low).requires_grad_(True)
+        plain = w.detach().dequantize(low) if quantised else w.detach().to(low)
+        plain.requires_grad_(True)
+        want = linear_cross_entropy(c, plain, y)
+        want = (want, *torch.autograd.grad(want, (c, plain)))
+        with torch.autocast("cuda", dtype=low):
+            loss = linear_cross_entropy(x, w, y)
+        got = (loss, *torch.autograd.grad(loss, (x, w)))
+        assert all(v.dtype == torch.float32 for v in got)
+        assert all(torch.equal(i.float(), j.float()) for i, j in zip(got, want))
+
+
 def test_another_stream_and_repeated_calls():
     x, w, y = _inputs(300, 264, 2000, F16)
     one = torch.ones((), device="cuda")
