@@ -46,8 +46,9 @@ class _PlainTensorHooks:
                 unexpected_keys, error_msgs):
         suffixes = self.weight_cls.canonical_key_suffixes()
         found = {s: state_dict.pop(prefix + s) for s in suffixes if prefix + s in state_dict}
-        # a "weight" that is not codes is an ordinary checkpoint: put it back, copy_ re-quantises
-        if "weight" in found and found["weight"].dtype not in (torch.uint8, torch.float8_e4m3fn):
+        # a "weight" that is not this format's codes is an ordinary checkpoint: put it back,
+        # copy_ re-quantises
+        if "weight" in found and found["weight"].dtype not in self.weight_cls._CODE_DTYPES:
             state_dict[prefix + "weight"] = found.pop("weight")
         if not found:
             return

@@ -121,6 +121,7 @@ class QWeightBase(Tensor):
     """
 
     _PAYLOAD: tuple = ()
+    _CODE_DTYPES = (torch.uint8,)  # of a checkpoint's "weight" that is not one of values
     _ATEN_OP_TABLE: dict
     _TORCH_FN_TABLE: dict
 

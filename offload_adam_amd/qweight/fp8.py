@@ -159,6 +159,7 @@ class FP8QWeight(QWeightBase):
     re-quantises in place."""
 
     _PAYLOAD = ("weight", "block_scale")
+    _CODE_DTYPES = (torch.float8_e4m3fn, torch.uint8)  # the latter are refused
 
     @staticmethod
     @torch._dynamo.disable

@@ -215,6 +215,19 @@ def test_checkpoints_with_other_scales_are_encoded_again():
         FP8QWeight.from_plain_state_dict({"weight": codes, "weight_scale_inv": scale})
 
 
+@pytest.mark.parametrize("name", ["int8", "int4", "nf4", "nvfp4"])
+def test_other_formats_take_float8_weights_as_values(name):
+    g = torch.Generator().manual_seed(5)
+    model = nn.Sequential(nn.Linear(128, 64, bias=False)).to(BF16)
+    quantize_linears(model, FORMATS[name])
+    values = torch.randn(64, 128, generator=g).to(torch.float8_e4m3fn)
+    model.load_state_dict({"0.weight": values})
+    want = FORMATS[name].from_float(torch.zeros(64, 128, dtype=BF16))
+    want.copy_(values)
+    assert torch.equal(model[0].weight.data.dequantize(torch.float32),
+                       want.dequantize(torch.float32))
+
+
 @pytest.mark.parametrize("power", [False, True])
 def test_checkpoints_that_do_not_fit_are_refused(power):
     """Scales of finer, coarser or transposed blocks, or that are no scales; codes of another
@@ -240,6 +253,8 @@ def test_checkpoints_that_do_not_fit_are_refused(power):
         with pytest.raises(ValueError, match="weight_scale_inv"):
             load(codes, scale)
     for weight in (codes.view(torch.uint8), codes.to(torch.float8_e5m2), codes[:, :250], codes[0]):
+        with pytest.raises(ValueError, match="weight must be"):
+            load(codes.view(torch.uint8), scales(3, 2))
         with pytest.raises(ValueError, match="weight must be"):
             FP8QWeight.from_plain_state_dict({"weight": weight, "weight_scale_inv": scales(3, 2)},
                                              model[0].weight.data)
