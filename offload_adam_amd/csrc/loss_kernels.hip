@@ -286,7 +286,7 @@ ce_reduce_kernel(const float* __restrict__ block_sum, const int* __restrict__ bl
 // of their size, 1.7e-3 of it the rounding of the results, against 2.6e-3).  One g per
 // token, bf16: d is stored times g, and everything else is 1.  fp16, whose smallest normal
 // number (6e-5) is far above a probability times a gradient of 1 / tokens: g = top m 2^e
-// with top the largest |g| of all tokens and 1/2 < |m| <= 1; d is stored times 2^15 m, x
+// with top the largest finite |g| of all tokens and 1/2 < |m| <= 1; d is stored times 2^15 m, x
 // times 2^e (exactly, but for its smallest numbers), and the rest goes into the fp32 sums.
 struct TokenFactors {
   float* d;   // of d as it is stored; 0: the token takes no part
@@ -361,16 +361,22 @@ ce_factors_kernel(const Gradient a, const TokenFactors f) {
   for (int64_t i = threadIdx.x; i < a.tokens; i += kReduceThreads) {
     const float g = a.takes_part(i) ? a.grad[i] + a.fault(i) : 0.0f;
     f.d[i] = g;
-    top = fmaxf(top, fabsf(g));
+    if (fabsf(g) < INFINITY) top = fmaxf(top, fabsf(g));
   }
   top = wave_max(top);
   if (threadIdx.x % kWave == 0) tops[threadIdx.x / kWave] = top;
   __syncthreads();
   for (int w = 0; w < kReduceThreads / kWave; ++w) top = fmaxf(top, tops[w]);
+  if (top == 0.0f) top = 1.0f;
   if (threadIdx.x == 0) *f.dw = top / kF16Lift;
   // each lane goes over what it wrote itself
   for (int64_t i = threadIdx.x; i < a.tokens; i += kReduceThreads) {
     const float g = f.d[i];
+    if (!(fabsf(g) < INFINITY)) {  // infinities and NaN stay in their row of dx
+      f.d[i] = g;
+      f.x[i] = f.dx[i] = 1.0f;
+      continue;
+    }
     int e = 0;
     float m = g == 0.0f ? 0.0f : frexpf(g / top, &e);
     if (fabsf(m) == 0.5f) {

@@ -287,6 +287,28 @@ def test_tokens_whose_gradient_is_zero(dtype, reduction):
         assert not dx.any() and not dw.any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_that_are_not_finite_stay_in_their_rows(dtype):
+    x, w, y = _inputs(140, 72, 500, dtype, seed=7, ignore_index=7)
+    y[:4] = 3
+    grad = _grad_for("none", 140)
+    clean = _run(x, w, y, grad, reduction="none", ignore_index=7)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        grad[[1, 3]] = bad
+        loss, dx, dw = _run(x, w, y, grad, reduction="none", ignore_index=7)
+        assert torch.equal(loss, clean[0])
+        assert not torch.isfinite(dx[[1, 3]]).all(1).any() and not torch.isfinite(dw).all()
+        # the largest gradient of the others is the same: so is what it scales
+        rest = grad.clone()
+        rest[[1, 3]] = 0.0
+        want = _run(x, w, y, rest, reduction="none", ignore_index=7)[1]
+        keep = torch.ones(140, dtype=torch.bool, device="cuda")
+        keep[[1, 3]] = False
+        assert torch.equal(dx[keep], want[keep]) and torch.isfinite(want).all()
+    grad[:] = float("inf")  # nothing finite to scale by
+    assert not torch.isfinite(_run(x, w, y, grad, reduction="none", ignore_index=7)[2]).all()
+
+
 def test_gradient_against_differences():
     """Along a direction s of +-1 with steps that 16-bit numbers hold exactly.  The
     third derivative along s is a third cumulant of the logits' direction, at most the
