@@ -385,8 +385,8 @@ ce_factors_kernel(const Gradient a, const TokenFactors f) {
     }
     const float power = ldexpf(1.0f, e);
     f.d[i] = m * kF16Lift;
-    f.x[i] = g == 0.0f ? 0.0f : power;
-    f.dx[i] = top * power / kF16Lift;
+    f.x[i] = m == 0.0f ? 0.0f : power;
+    f.dx[i] = m == 0.0f ? 0.0f : top * power / kF16Lift;
   }
 }
 

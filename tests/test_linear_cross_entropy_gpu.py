@@ -309,6 +309,24 @@ def test_gradients_that_are_not_finite_stay_in_their_rows(dtype):
     assert not torch.isfinite(_run(x, w, y, grad, reduction="none", ignore_index=7)[2]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("shape", [(140, 72, 500), (300, 512, 400), (3, 64, 9000)])
+def test_tokens_that_take_no_part_meet_a_head_that_is_not_finite(shape, reduction, dtype):
+    x, w, y = _inputs(*shape, dtype, seed=8, ignore=0.5)
+    y[0], y[-1] = -100, 0
+    w[3, 5], w[7, 0] = float("inf"), float("nan")
+    grad = _grad_for(reduction, shape[0])
+    out = y == -100
+    if reduction == "none":
+        grad[1] = 0.0
+        out[1] = True
+    loss, dx, _ = _run(x, w, y, grad, reduction=reduction)
+    assert not dx[out].any() and not torch.isfinite(dx[~out]).all(1).any()
+    if reduction == "none":
+        assert not loss[y == -100].any()
+
+
 def test_gradient_against_differences():
     """Along a direction s of +-1 with steps that 16-bit numbers hold exactly.  The
     third derivative along s is a third cumulant of the logits' direction, at most the
