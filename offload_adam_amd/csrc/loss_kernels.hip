@@ -285,9 +285,14 @@ ce_reduce_kernel(const float* __restrict__ block_sum, const int* __restrict__ bl
 // (98 tokens, 31151 words, random logits, a sum times a random g: gradients off by 1.9e-3
 // of their size, 1.7e-3 of it the rounding of the results, against 2.6e-3).  One g per
 // token, bf16: d is stored times g, and everything else is 1.  fp16, whose smallest normal
-// number (6e-5) is far above a probability times a gradient of 1 / tokens: g = top m 2^e
-// with top the largest finite |g| of all tokens and 1/2 < |m| <= 1; d is stored times 2^15 m, x
-// times 2^e (exactly, but for its smallest numbers), and the rest goes into the fp32 sums.
+// number (6e-5) is far above a probability times a gradient of 1 / tokens: g = top m 2^(a + b)
+// with top the largest finite |g| of all tokens and 1/2 < |m| <= 1; d is stored times
+// 2^15 m 2^a, x times 2^b, and the rest goes into the fp32 sums.  Both are exact but for
+// fp16's smallest step, 2^-25 off at most: 2^(-40 - a) of d and 2^(-25 - b) of x.  So b goes
+// down to -8 first, x then being exact from 2^-6 on, then a to -12, where the error of d
+// is 2^-28 (of 131072 probabilities together no more than the rounding of the target's
+// element), and b takes what is left under 2^-20.  (All of it in b left x four of its eleven
+// bits at 2^-20.)
 struct TokenFactors {
   float* d;   // of d as it is stored; 0: the token takes no part
   float* x;   // of x for dw
@@ -383,8 +388,9 @@ ce_factors_kernel(const Gradient a, const TokenFactors f) {
       m *= 2.0f;
       e -= 1;
     }
-    const float power = ldexpf(1.0f, e);
-    f.d[i] = m * kF16Lift;
+    const int a = e > -8 ? 0 : e < -20 ? -12 : e + 8;
+    const float power = ldexpf(1.0f, e - a);
+    f.d[i] = ldexpf(m * kF16Lift, a);
     f.x[i] = m == 0.0f ? 0.0f : power;
     f.dx[i] = m == 0.0f ? 0.0f : top * power / kF16Lift;
   }

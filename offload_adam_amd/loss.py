@@ -117,7 +117,9 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     ``reduction``: ``"mean"`` over the tokens that take part (NaN if there are none),
     ``"sum"``, or ``"none"`` (losses of ``target``'s shape).  The loss is fp32;
     logits, exponentials and sums are fp32 throughout, and only the logits' gradient is
-    rounded to 16 bits, once, between the two products that use it.  Gradients flow to
+    rounded to 16 bits, once, between the two products that use it.  (fp16 with a gradient
+    per token: hidden states enter the weight's gradient scaled by a power of two, off by
+    2^-17 at most for tokens whose gradient is 2^-20 of the largest or more.)  Gradients flow to
     ``x`` and ``weight``; taking second derivatives or forward-mode ones raises.  Results
     do not depend on anything but the arguments: no atomics, one order of summation.
 

@@ -327,6 +327,52 @@ def test_tokens_that_take_no_part_meet_a_head_that_is_not_finite(shape, reductio
         assert not loss[y == -100].any()
 
 
+@pytest.mark.parametrize("low", [-4, -8, -13, -20])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_of_very_different_size(dtype, low):
+    """Words that only tokens of small gradients know of: their rows of dw, and those tokens'
+    rows of dx, as exact as the large ones.  fp16 holds d under a lift of 2^15, of which a
+    small gradient takes up to 2^12, and x times 2^-8 or more: half of its smallest step, 2^-25,
+    is 2^-40 of d (small gradients: 2^-28) and 2^-17 of x."""
+    t, h, v = 96, 64, 300
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(t, h, generator=g)
+    w = torch.randn(v, h, generator=g) / 4
+    x[:, 0] = torch.where(torch.arange(t) < t // 2, 8.0, -8.0)
+    w[:, 0] = torch.where(torch.arange(v) < v // 2, 8.0, -8.0)  # the other half: e^-128 less
+    x, w = x.to(dtype).cuda(), w.to(dtype).cuda()
+    y = torch.cat((torch.randint(v // 2, (t // 2,), generator=g),
+                   torch.randint(v // 2, v, (t // 2,), generator=g))).cuda()
+    grad = (torch.rand(t, generator=g) + 0.5).cuda() * 2.0**12
+    grad[t // 2:] *= 2.0**low
+    _, dx, dw = _run(x, w, y, grad, reduction="none")
+    r = torch.finfo(dtype).eps / 2
+    xd, wd, up = x.double(), w.double(), grad.double()[:, None]
+    z = xd @ wd.t().contiguous()
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    d = p.scatter_add(1, y[:, None], torch.full_like(p[:, :1], -1.0))
+    dz = (xd.abs() @ wd.abs().t().contiguous()).amax(1, keepdim=True) * h * 2 * U
+    rel = 2 * dz + 256 * U + 16 * U * (lse.abs() + z.abs().amax(1, keepdim=True))
+    err = p * rel + d.abs() * (r + 2 * U) + 2.0**-126
+    off_x = torch.zeros(())
+    if dtype == F16:
+        err = err + torch.where(torch.arange(t) < t // 2, 2.0**-40, 2.0**-28)[:, None].cuda()
+        off_x = 2.0**-17 * (d.abs() * up).sum(0)[:, None]
+    floor = 2.0**-24 if dtype == F16 else 2.0**-126
+    want = (d * up) @ wd
+    tol = up * ((err + d.abs() * (v + 8) * 2 * U) @ wd.abs()) + want.abs() * r + floor
+    _close(dx, (want, tol), "dx")
+    du = (d * up).t().contiguous()
+    want = du @ xd
+    tol = (err * up).t().contiguous() @ xd.abs() + du.abs() @ xd.abs() * (t + 8) * 2 * U
+    tol = tol + off_x.cuda() + want.abs() * r + floor
+    # two tokens of one word: 2 * 8 * 6144 = 98304 in column 0, over fp16's 65504
+    fits = want.abs() + tol < torch.finfo(dtype).max
+    assert fits[:, 1:].all() and torch.equal(torch.isinf(dw), ~fits)
+    _close(dw[fits], (want[fits], tol[fits]), "dw")
+
+
 def test_gradient_against_differences():
     """Along a direction s of +-1 with steps that 16-bit numbers hold exactly.  The
     third derivative along s is a third cumulant of the logits' direction, at most the
