@@ -37,6 +37,13 @@ constexpr int kReduceThreads = 1024;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// exp(z - m) is exp2(fma(z, log2e, -at)) * unrounded(m, at) with at = m * log2e rounded: one
+// fma per logit, and what the rounding of `at` makes of all of a token's exponentials (2^-24 of
+// |m|) is taken back once.
+__device__ __forceinline__ float unrounded(float m, float at) {
+  return fabsf(at) < INFINITY ? exp2_hw(-fmaf(m, kLog2e, -at)) : 1.0f;
+}
+
 // (maximum, sum of exp(z - maximum)) of two disjoint sets of logits.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
@@ -120,12 +127,13 @@ struct StatsEpilogue {
       for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = fmaxf(m, t.quad(u, b)[i]);
-      const float at = (m == -INFINITY ? 0.0f : m) * kLog2e;
+      const float from = m == -INFINITY ? 0.0f : m, at = from * kLog2e;
       float s = 0.0f;
 #pragma unroll
       for (int u = 0; u < Tl::kQuads; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s += exp2_hw(fmaf(t.quad(u, b)[i], kLog2e, -at));
+      s *= unrounded(from, at);
       const int64_t y = token < tokens ? target[token] : -1;
       const int rel = column_of<Tl>(y < vocab ? y - v0 : -1);
       if (__any(rel >= 0)) {
@@ -157,11 +165,12 @@ struct Losses {
   // A token whose logits have this maximum and sum: its loss, 0 if it takes no part.  A
   // target outside [0, vocab) that is not `ignore` makes it NaN.
   __device__ __forceinline__ float finish(int64_t token, float m, float s, bool& used) const {
-    const float l = m + logf(s);
-    lse[token] = l;
+    const float l = logf(s);
+    lse[token] = m + l;
     const int64_t y = target[token];
     used = y != ignore;
-    const float v = !used ? 0.0f : y >= 0 && y < vocab ? l - z_target[token] : NAN;
+    // the difference of the large ones first: l alone is as small as the loss may be
+    const float v = !used ? 0.0f : y >= 0 && y < vocab ? m - z_target[token] + l : NAN;
     if (loss) loss[token] = v;
     return v;
   }
@@ -418,8 +427,10 @@ struct ProbEpilogue {
     for (int b = 0; b < Tl::kColumns; ++b) {
       const int64_t token = row_p + t.p0() + kLines * b;
       const bool here = token < tokens;
+      const float l = here ? lse[token] : 0.0f;
       h[b] = here ? factor[token] : 0.0f;
-      at[b] = (here ? lse[token] : 0.0f) * kLog2e;
+      at[b] = l * kLog2e;
+      if (h[b] != 0.0f) h[b] *= unrounded(l, at[b]);
     }
     auto p = [&](float z, int b) { return exp2_hw(fmaf(z, kLog2e, -at[b])); };
     t.rows16(
@@ -439,8 +450,11 @@ struct ProbEpilogue {
             const int rel = column_of<Tl>(y < rows ? y - v0 : -1);
             if (!__any(rel >= 0)) continue;
             const float z = logit_at(t, b, rel);
-            if (rel >= 0 && h[b] != 0.0f)
-              t.put16(lds, rel, b, (uint16_t)Store16<T>::pack((p(z, b) - 1.0f) * h[b], 0.0f));
+            if (rel >= 0 && h[b] != 0.0f) {
+              const float one = p(z, b) * unrounded(lse[token], at[b]);  // or less
+              t.put16(lds, rel, b,
+                      (uint16_t)Store16<T>::pack((one - 1.0f) * factor[token], 0.0f));
+            }
           }
         },
         [&](int p, int q, u32x4 v) {

@@ -163,6 +163,37 @@ def test_large_logits_and_confident_rows():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+def test_exact_logits_of_thousands(dtype):
+    """Logits up to 6000 that fp32 holds exactly, so that all that is left is the exponentials'
+    exponents (under 64 in base 2 where they count: 2^-24 of 64 each way, and as much again
+    for log2 e), the sum and the logarithm.  First the target far above all others: loss and
+    gradients 0 but for two exponentials and a product of 1 +- 2^-23.  Then 16 equal logits at
+    the top and the others 1 to 40 below."""
+    t, v, h = 130, 300, 16
+    g = torch.Generator().manual_seed(11)
+    top = torch.randint(33, 96, (t,), generator=g).float()  # times 64: 2112 to 6080
+    x = torch.zeros(t, h)
+    x[:, 0], x[:, 1] = top, 1.0
+    w = torch.zeros(v, h)
+    w[:, 0] = 64.0
+    for far in (True, False):
+        w[:, 1] = -torch.randint(200, 250, (v,), generator=g) if far else \
+            -torch.randint(1, 41, (v,), generator=g)
+        same = 1 if far else 16
+        w[100:100 + same, 1] = 0.0
+        y = torch.full((t,), 100)
+        a, b = x.to(dtype).cuda(), w.to(dtype).cuda()
+        loss, dx, dw = _run(a, b, y.cuda(), torch.ones(t, device="cuda"), reduction="none")
+        z = (x.double() @ w.double().t())
+        want = torch.logsumexp(z, 1) - z[:, 100]
+        tol = 2.0**-16 if not far else 2.0**-21
+        assert float((loss.cpu().double() - want).abs().max()) <= tol
+        if far:
+            assert float(dx[:, 0].abs().max()) <= 2.0**-21 * 64
+            assert float(dw[100, 0].abs()) <= 2.0**-21 * float(top.sum())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 def test_ignored_rows_may_hold_anything(dtype):
     t, h, v = 150, 88, 400
     x, w, y = _inputs(t, h, v, dtype, seed=4, ignore_index=7)
