@@ -41,6 +41,7 @@ HIPCC_FLAGS = [
     "-Xclang",
     "-packed-fp32-ops",
     "-Wall",
+    "-Werror=inline-asm",
     "-Wno-unused-function",
     "-Wno-unknown-warning-option",
 ]
