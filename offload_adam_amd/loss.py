@@ -18,14 +18,14 @@ _CASTABLE = (torch.float32, torch.float16, torch.bfloat16)
 _REDUCTIONS = {"none": _lib.OA_LOSS_NONE, "mean": _lib.OA_LOSS_MEAN, "sum": _lib.OA_LOSS_SUM}
 
 
-def _rows(t, name):
+def _rows(t):
     """2-D operand of the kernels: unit column stride, columns and row stride multiples
     of 8 elements, 16-byte aligned.  Anything else is copied, zero-padded."""
     rows, cols = t.shape
     if cols % 8 == 0 and cols <= 1 << 20 and t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t, cols, cols
     stride = t.stride(0) if rows > 1 else -(-cols // 8) * 8
-    if (cols % 8 == 0 and (cols == 1 or t.stride(1) == 1) and stride >= cols and stride % 8 == 0
+    if (cols % 8 == 0 and t.stride(1) == 1 and stride >= cols and stride % 8 == 0
             and stride <= 1 << 20 and t.data_ptr() % 16 == 0):
         return t, cols, stride
     padded = -(-cols // 8) * 8
@@ -41,8 +41,8 @@ def _plain(weight, dtype):
 
 
 def _head_args(x, w, target, ignore_index, reduction):
-    x, hidden, ldx = _rows(x, "x")
-    w, _, ldw = _rows(w, "weight")
+    x, hidden, ldx = _rows(x)
+    w, _, ldw = _rows(w)
     args = [x.data_ptr(), ldx, w.data_ptr(), ldw, _lib.dtype_code(x.dtype), target.data_ptr(),
             x.shape[0], hidden, w.shape[0], ignore_index, _REDUCTIONS[reduction]]
     return args, hidden, (x, w)
