@@ -73,6 +73,51 @@ def test_strided_sources_and_in_place():
         q.copy_(torch.zeros(3, 16, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("stride, first", [(272, 0), (280, 8), (281, 0), (300, 3)])
+def test_the_c_decoder_writes_rows_of_any_stride_and_alignment(stride, first, dtype):
+    """Rows that 16-byte stores fit, and rows that take single elements; nothing beside them."""
+    from offload_adam_amd import _lib
+    from offload_adam_amd.qweight import FP8QWeight
+
+    rows, cols = 131, 272
+    q = FP8QWeight.from_float(awkward(rows, cols, seed=2).cuda())
+    out = torch.full((rows * stride + 16,), 7.0, dtype=dtype, device="cuda")
+    want = out.clone()
+    want[first:first + rows * stride].view(rows, stride)[:, :cols] = q.dequantize(dtype)
+    code = _lib.load().oa_dequant_fp8(
+        q.weight.data_ptr(), q.block_scale.data_ptr(), rows, cols,
+        out.data_ptr() + first * out.element_size(), _lib.dtype_code(dtype), stride,
+        _lib.current_stream_ptr())
+    assert code == 0 and _same(out, want)
+
+
+def test_state_dict_on_the_gpu():
+    from offload_adam_amd.qweight import FP8QWeight, quantize_linears
+
+    g = torch.Generator().manual_seed(1)
+    model = nn.Sequential(nn.Linear(272, 200, bias=False)).to(BF16).cuda()
+    other = nn.Sequential(nn.Linear(272, 200, bias=False)).to(BF16).cuda()
+    for m in (model, other):
+        quantize_linears(m, FP8QWeight)
+    sd = model.state_dict()
+    for checkpoint in (sd, {k: v.cpu() for k, v in sd.items()}):
+        other[0].weight.data.copy_(torch.zeros(200, 272, device="cuda"))
+        other.load_state_dict(checkpoint)
+        assert torch.equal(_bits(other[0].weight.data.weight), _bits(model[0].weight.data.weight))
+        assert torch.equal(_bits(other[0].weight.data.block_scale),
+                           _bits(model[0].weight.data.block_scale))
+    scale = torch.rand(2, 3, generator=g) + 0.3
+    codes = torch.randn(200, 272, generator=g).mul(50).to(torch.float8_e4m3fn)
+    loaded = []
+    for device in ("cpu", "cuda"):
+        other.load_state_dict({"0.weight": codes.to(device), "0.weight_scale_inv": scale.to(device)})
+        loaded.append(other[0].weight.data.dequantize(F32).cpu())
+    spread = scale.repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)[:, :272]
+    want = FP8QWeight.from_float(codes.float() * spread).dequantize(F32)
+    assert torch.equal(loaded[0], want) and torch.equal(loaded[1], want)
+
+
 def test_codec_on_more_than_2_31_elements():
     from offload_adam_amd.qweight import FP8QWeight
 
