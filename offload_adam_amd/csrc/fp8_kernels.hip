@@ -690,10 +690,8 @@ void launch_few(const Few<DT>& a, int waves, hipStream_t s) {
   const dim3 grid((unsigned)tiles_along(a.out_f, kLines)), block(waves * kWave);
   if (waves == 4)
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 4, ENCODE>), grid, block, 0, s, a);
-  else if (waves == 8)
+  else
     hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 8, ENCODE>), grid, block, 0, s, a);
-  else if constexpr (ENCODE)
-    hipLaunchKernelGGL((fp8_few_kernel<DT, TILES, 16, ENCODE>), grid, block, 0, s, a);
 }
 
 // Slices of the cut tiles -> results, four columns of a row per lane.
@@ -801,20 +799,19 @@ struct Layer {
 
 // Whether the kernel for few tokens takes a call.  It reads every token's codes once per 16
 // columns, the tiles once per 128, but those take two more launches and half the bytes they
-// move in LDS are for rows that hold no token.  4096 -> 14336: 15, 17 and 23 us for 1, 4 and
-// 16 tokens, 22 with tiles; 28 against 22 for 24; a small weight gains for longer: 4096 ->
-// 4096, 24 tokens, 11 against 15.
+// move in LDS are for rows that hold no token.  Weights that come from HBM, bf16: 14336 -> 4096,
+// 13 and 21 us for 1 and 16 tokens, 23 and 24 with tiles; 4096 -> 14336, 14 and 22 against 22
+// and 22; beyond 16 tokens, 4096 -> 14336, 27 against 20 for 24, but a small weight gains for
+// longer: 4096 -> 4096, 10 against 13.  Only very wide weights turn earlier: 4096 -> 128256,
+// 101 against 114 for 4 tokens, 124 against 114 for 8.
 bool takes_few(const Layer& w, int64_t tokens) {
   return tokens <= kLines || (tokens <= 2 * kLines && w.out_f * w.in_f <= (1 << 24));
 }
 // Waves of its workgroups: a CU that has only one of them needs more loads in flight from
-// it.  1 token, 4 / 8 / 16 waves: 4096 -> 14336, 14.6, 14.1, 19.6 us; 2048 -> 5632, 5.3, 6.0,
-// 8.6; 4096 -> 4096, 6.1, 5.7, 6.2; 14336 -> 4096, 13.8, 13.5, 12.9.  8 tokens: 4096 ->
-// 14336, 20.8, 21.1, 25.2; 14336 -> 4096, 21.5, 18.3, 19.3.
-int few_waves(const Layer& w, bool encode) {
-  if (tiles_along(w.out_f, kLines) > 256) return 4;
-  return encode && blocks_of(w.in_f) >= 64 ? 16 : 8;
-}
+// it.  4 / 8 waves, weights that come from HBM, bf16, 1 token: 4096 -> 14336, 14.4, 14.3 us;
+// 2048 -> 5632, 5.5, 6.3; 4096 -> 4096, 6.3, 6.0; 14336 -> 4096, 13.4, 13.2; 2 tokens there,
+// 19.3, 16.0; 8 tokens: 4096 -> 14336, 19.7, 21.1; 14336 -> 4096, 19.9, 18.2.
+int few_waves(const Layer& w) { return tiles_along(w.out_f, kLines) > 256 ? 4 : 8; }
 
 struct ForwardPlan {
   Encoded x{};
@@ -838,7 +835,7 @@ int forward(const Source& x, const Layer& w, const void* bias, void* y, void* ws
   if (few) {
     const int tokens = (int)x.rows;
     const bool encode = tokens <= kFewEncodeTokens && tokens * plan.x.ld <= kFewCodes;
-    const int waves = few_waves(w, encode);
+    const int waves = few_waves(w);
     const Few<DT> a{w.q, w.scales, w.out_f, (int)w.in_f, (int)blocks_of(w.in_f),
                     x, plan.x.q, plan.x.scales, plan.x.ld,
                     plan.x.scale_stride, tokens, bias, y};
