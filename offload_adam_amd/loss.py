@@ -76,8 +76,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     @_qbase.first_derivatives_only
-    def backward(ctx, grad):
-        x, weight, target, stats = ctx.saved_tensors
+    def backward(ctx, saved, grad):
+        x, weight, target, stats = saved
         want_dx, want_dw = ctx.needs_input_grad[:2]
         tokens, dev = x.shape[0], x.device
         if tokens == 0:

@@ -70,18 +70,20 @@ class _Refusal(torch.autograd.Function):
 
 
 def first_derivatives_only(backward):
-    """Decorator of a function's ``backward`` that is not differentiable.  With
+    """Decorator of a function's ``backward(ctx, saved, *grads)`` that is not
+    differentiable; ``saved``: the saved tensors, which checkpointing hands out once.  With
     ``create_graph`` its results hang on everything they were computed from, so that a
     second derivative raises; ``once_differentiable`` lets it be zero where the incoming
     gradient is a constant or is what it is taken by."""
 
     @functools.wraps(backward)
     def wrapper(ctx, *grads):
+        saved = ctx.saved_tensors
         with torch.no_grad():
-            out = backward(ctx, *grads)
+            out = backward(ctx, saved, *grads)
         if not torch.is_grad_enabled():
             return out
-        return _Refusal.apply(len(out), *out, *grads, *ctx.saved_tensors)
+        return _Refusal.apply(len(out), *out, *grads, *saved)
 
     return wrapper
 

@@ -134,8 +134,8 @@ class _FP8Linear(torch.autograd.Function):
 
     @staticmethod
     @first_derivatives_only
-    def backward(ctx, grad):
-        x, weight = ctx.saved_tensors
+    def backward(ctx, saved, grad):
+        x, weight = saved
         want_dx, want_dw, want_db = ctx.needs_input_grad
         flat, g = _rows_of(x), _rows_of(grad)
         if x.is_cuda:

@@ -9,6 +9,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
+from torch.utils.checkpoint import checkpoint
 
 from offload_adam_amd import _lib
 from offload_adam_amd.qweight import FORMATS, FP8QWeight, quantize_linears
@@ -97,6 +98,16 @@ def test_linear_and_its_gradients():
     assert (dx.reshape(-1, 144).double() - held(gy, 1, 128) @ wv).abs().max() < 210 * 2**-23 * 600
     assert (dw.double() - held(gy, 128, 1).T @ held(flat, 128, 1)).abs().max() < 210 * 2**-23 * 600
     assert (db.double() - gy.double().sum(0)).abs().max() < 210 * 2**-23 * 210
+
+
+def test_checkpointing_with_create_graph():
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(4, 64, generator=g).requires_grad_(True)
+    w = nn.Parameter(FP8QWeight.from_float(torch.randn(32, 64, generator=g)))
+    want = torch.autograd.grad(F.linear(x, w).sum(), (x, w))
+    y = checkpoint(F.linear, x, w, use_reentrant=False)
+    dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert torch.equal(dx, want[0])
 
 
 def test_forward_mode_is_refused():
