@@ -11,8 +11,8 @@
 //   dw = gt^T xt     gt, xt: blocks of 128 x 1 along the tokens  (T x N)^T (T x K)
 //
 // Products accumulate in fp32 and are rounded once, to the type of x.  4096 tokens, 4096 ->
-// 14336, bf16: forward 13 us to encode x and 207 to 227 for y (2.1 to 2.3 PFLOP/s); backward
-// 59 to encode, 175 to 200 for dx, 193 to 240 for dw, by the clock that power allows.
+// 14336, bf16: forward 13 us to encode x and 206 to 230 for y (2.1 to 2.3 PFLOP/s); backward
+// 60 to encode, 174 to 195 for dx, 193 to 230 for dw, by the clock that power allows.
 
 #include <math.h>
 

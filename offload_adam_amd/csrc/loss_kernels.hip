@@ -11,11 +11,12 @@
 // lie (line by line along the dimension that is summed over).
 //
 // Bound by the matrix cores: 2 T V H operations forward, 6 T V H backward (z is
-// computed again).  4096 tokens, 2048 hidden, 32000 words, bf16: 410 to 470 us forward;
-// backward, in two pieces, each 230 to 265 for d, 186 to 230 for dx and 195 to 225 for dw, by
+// computed again).  4096 tokens, 2048 hidden, 32000 words, bf16: 410 to 475 us forward;
+// backward, in two pieces, each 213 to 260 for d, 182 to 230 for dx and 195 to 225 for dw, by
 // the clock that power allows.  Logits, maxima, sums and the sums over tokens and vocabulary are
-// fp32; d is rounded once to the 16-bit type of x and W, which the products need and which
-// a framework that stores the logits' gradient does too.
+// fp32; lse_t is one fp32 number, which makes d off by 2^-24 of its magnitude; d is rounded once
+// to the 16-bit type of x and W, which the products need and which a framework that stores the
+// logits' gradient does too.
 
 #include <math.h>
 
