@@ -133,9 +133,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     decoded = weight.dtype
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    kind = x.device.type
-    if torch.is_autocast_enabled(kind):  # what F.linear casts
-        low = torch.get_autocast_dtype(kind)
+    low = _qbase.autocast_dtype(x)
+    if low is not None:  # what F.linear casts
         if x.dtype in _CASTABLE:
             x = x.to(low)
         if weight.dtype in _CASTABLE:

@@ -57,6 +57,14 @@ def _dequantized(weight, dtype):
     return w
 
 
+def autocast_dtype(t):
+    """What autocast casts an operand on ``t``'s device to; None where it is off or unknown."""
+    kind = t.device.type
+    if kind in ("cuda", "cpu") and torch.is_autocast_enabled(kind):
+        return torch.get_autocast_dtype(kind)
+    return None
+
+
 class _Refusal(torch.autograd.Function):
     """The first ``count`` tensors, on which differentiating by any of the others fails."""
 

@@ -37,7 +37,7 @@ from torch import Tensor
 from torch.autograd import forward_ad
 
 from . import _codec_ops
-from .base import QWeightBase, first_derivatives_only
+from .base import QWeightBase, autocast_dtype, first_derivatives_only
 
 FP8_BLOCK = _codec_ops.FP8_BLOCK
 FP8_E4M3_MAX = 448.0
@@ -274,9 +274,9 @@ def _linear(func, types, args, kwargs):
                              f"{tuple(codes.shape)} do not match")
         if input.device != codes.device:
             raise ValueError(f"linear: input is on {input.device}, weight on {codes.device}")
-        kind = input.device.type
-        if torch.is_autocast_enabled(kind):  # as for a plain weight
-            input = input.to(torch.get_autocast_dtype(kind))
+        low = autocast_dtype(input)
+        if low is not None:  # as for a plain weight
+            input = input.to(low)
         if bias is not None:
             if tuple(bias.shape) != (codes.shape[0],) or bias.device != input.device:
                 raise ValueError(f"linear: bias must have shape ({codes.shape[0]},) on "

@@ -110,6 +110,15 @@ def test_checkpointing_with_create_graph():
     assert torch.equal(dx, want[0])
 
 
+def test_shapes_on_the_meta_device():
+    w = FP8QWeight.from_float(torch.randn(32, 64, device="meta"))
+    x = torch.randn(2, 3, 64, device="meta")
+    for enabled in (False, True):
+        with torch.autocast("cpu", dtype=BF16, enabled=enabled):
+            y = F.linear(x, w, torch.zeros(32, device="meta"))
+        assert y.shape == (2, 3, 32) and y.dtype == torch.float32 and y.device.type == "meta"
+
+
 def test_forward_mode_is_refused():
     """A layer that nothing requires a gradient of has no tangents either, as the other
     formats' layers."""

@@ -55,6 +55,11 @@ def test_autocast_casts_before_the_checks():
         linear_cross_entropy(x.to(BF16), FP8QWeight.from_float(w), y)
 
 
+def test_the_meta_device_is_refused_too():
+    with pytest.raises(ValueError, match="must be a GPU tensor"):
+        linear_cross_entropy(*(t.to("meta") for t in _args()))
+
+
 def test_the_c_entry_points_refuse_before_any_launch():
     lib = _lib.load()
     buf = (ctypes.c_char * 4096)()
