@@ -133,6 +133,9 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     decoded = weight.dtype
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    ignore_index = int(ignore_index)
+    if not -2**63 <= ignore_index < 2**63:
+        raise ValueError(f"ignore_index must be an int64, got {ignore_index}")
     low = _qbase.autocast_dtype(x)
     if low is not None:  # what F.linear casts
         if x.dtype in _CASTABLE:
@@ -160,5 +163,5 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     flat, rows = target, x
     if target.dim() != 1:
         flat, rows = target.reshape(-1), x.reshape(-1, x.shape[-1])
-    loss = _LinearCrossEntropy.apply(rows, weight, flat.contiguous(), int(ignore_index), reduction)
+    loss = _LinearCrossEntropy.apply(rows, weight, flat.contiguous(), ignore_index, reduction)
     return loss.reshape(target.shape) if reduction == "none" else loss

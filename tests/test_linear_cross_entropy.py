@@ -55,6 +55,16 @@ def test_autocast_casts_before_the_checks():
         linear_cross_entropy(x.to(BF16), FP8QWeight.from_float(w), y)
 
 
+def test_ignore_index_is_an_int64():
+    """Its low 64 bits would be another index."""
+    for bad in (2**63, 2**64 - 100, -2**63 - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            linear_cross_entropy(*_args(), ignore_index=bad)
+    for good in (2**63 - 1, -2**63, torch.tensor(3), True):
+        with pytest.raises(ValueError, match="must be a GPU tensor"):  # only that is left
+            linear_cross_entropy(*_args(), ignore_index=good)
+
+
 def test_the_meta_device_is_refused_too():
     with pytest.raises(ValueError, match="must be a GPU tensor"):
         linear_cross_entropy(*(t.to("meta") for t in _args()))
