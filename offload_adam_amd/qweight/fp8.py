@@ -193,8 +193,8 @@ class FP8QWeight(QWeightBase):
 
     @classmethod
     def can_quantize(cls, tensor: Tensor, **_) -> bool:
-        # rows of codes have to be whole 16-byte pieces
-        return tensor.dim() == 2 and tensor.shape[1] % 16 == 0
+        # rows of codes have to be whole 16-byte pieces, one at least for the products
+        return tensor.dim() == 2 and tensor.shape[1] % 16 == 0 and tensor.shape[1] > 0
 
     def _requantize_(self, src: Tensor) -> None:
         if self.weight.is_cuda:

@@ -235,6 +235,13 @@ def test_checkpoints_with_other_scales_are_encoded_again():
         FP8QWeight.from_plain_state_dict({"weight": codes, "weight_scale_inv": scale})
 
 
+def test_layers_without_inputs_stay_plain():
+    model = nn.Sequential(nn.Linear(0, 4), nn.Linear(16, 4))
+    report = quantize_linears(model, FP8QWeight)
+    assert report.quantized == ["1"] and report.incompatible[0][0] == "0"
+    assert torch.equal(model[0](torch.zeros(3, 0)), model[0].bias.expand(3, 4))
+
+
 @pytest.mark.parametrize("name", ["int8", "int4", "nf4", "nvfp4"])
 def test_other_formats_take_float8_weights_as_values(name):
     g = torch.Generator().manual_seed(5)
